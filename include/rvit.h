@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define RVIT_ABI_VERSION 29
+#define RVIT_ABI_VERSION 30
 
 #define RVIT_BF16 0
 #define RVIT_F32 1
@@ -637,6 +637,68 @@ int rvit_gru_step_fwd(const float* x, const float* w_ih, const float* w_hh, cons
                       float* saved, int B, int T, int In, int H, int step, void* stream);
 int rvit_gru_step_bwd(const float* dout, const float* w_hh_t, const float* w_hh_t_r, const float* saved, const float* out,
                       float* dgates, float* dh_carry, int B, int T, int H, int step, void* stream);
+
+/* ---- state-space sequence operators (vit_amd/ssm.py; the temporal encoder's model_type='ssm') ----------------------------
+ * Short causal convolution per channel: y[t] = act(bias + sum_k w[:, k] x[t - K + 1 + k]), 2 <= K <= 6, act = SiLU (silu != 0)
+ * or none.  x [B,T,C] (strides sxb, sxt in elements, channels packed), w fp32 [C,K], bias fp32 [C] or null; `state`
+ * [B,K-1,C] holds the inputs before the first token (null: zero), state_out receives the last K-1 before the end (may be null,
+ * may not be `state`).  lengths int32 [B] or null: sample b ends after lengths[b] tokens (clamped to 0..T); outputs and input
+ * gradients behind the end are zero, whatever the inputs hold there.  x, y, state of one dtype.  bwd: dw [C,K], dbias [C]
+ * fp32; dstate (gradient of `state`) and dstate_out (gradient of state_out) may be null.  step: one token, x [B,C], the kept
+ * inputs `state` advance in place. */
+int rvit_ssm_conv_fwd(const void* x, int64_t sxb, int64_t sxt, const float* w, const float* bias, const void* state,
+                      const int* lengths, void* y, void* state_out, int dtype, int B, int T, int C, int K, int silu,
+                      void* stream);
+int rvit_ssm_conv_bwd_workspace(int64_t* bytes, int B, int T, int C, int K);
+int rvit_ssm_conv_bwd(const void* x, int64_t sxb, int64_t sxt, const float* w, const float* bias, const void* state,
+                      const int* lengths, const void* dy, int64_t syb, int64_t syt, const void* dstate_out, void* dx,
+                      float* dw, float* dbias, void* dstate, void* workspace, int64_t workspace_bytes, int dtype, int B,
+                      int T, int C, int K, int silu, void* stream);
+int rvit_ssm_conv_step(const void* x, int64_t sxb, const float* w, const float* bias, void* state, void* y, int dtype, int B,
+                       int C, int K, int silu, void* stream);
+
+/* Selective scan: d = softplus(dt + dt_bias), S_t = exp(d_t A) S_{t-1} + d_t x_t B_t^T, y_t = (S_t C_t + D x_t) silu(z_t).
+ * x, z, y [B,T,H,P]; dt [B,T,H]; Bm, Cm [B,T,G,N] (shared by the H / G heads of a group), one dtype; A, D, dt_bias fp32 [H];
+ * states fp32 [B,H,P,N], 1 <= N <= 128.  Inputs have strides per sample and token in elements ([H,P], [G,N], [H] packed);
+ * outputs are packed.  D, z, dt_bias, state0, lengths, state_out may be null.  lengths as above: the returned state is the one
+ * behind the last token of each sample.  Training passes v (dtype, [B,T,H,P]; only with z) and states (fp32, state_floats of
+ * rvit_ssm_scan_plan), both read by bwd.  Workspaces: fwd_bytes / bwd_bytes of rvit_ssm_scan_plan, 16-byte aligned.  bwd:
+ * dA, dD, ddt_bias fp32 [H] (the last two may be null), dstate0 may be null, dz with z only.  Results do not depend on the
+ * order in which workgroups run.  A non-finite input of a valid token may reach every output of its chunk of 64 tokens.
+ * step: one token, x [B,H,P], state advances in place. */
+int rvit_ssm_scan_plan(int64_t* fwd_bytes, int64_t* state_floats, int64_t* bwd_bytes, int B, int T, int H, int P, int G,
+                       int N);
+int rvit_ssm_scan_fwd(const void* x, int64_t sxb, int64_t sxt, const void* dt, int64_t sdb, int64_t sdt, const float* A,
+                      const void* Bm, int64_t sbb, int64_t sbt, const void* Cm, int64_t scb, int64_t sct, const float* D,
+                      const void* z, int64_t szb, int64_t szt, const float* dt_bias, const float* state0, const int* lengths,
+                      void* y, void* v, float* state_out, float* states, void* workspace, int64_t workspace_bytes, int dtype,
+                      int B, int T, int H, int P, int G, int N, void* stream);
+int rvit_ssm_scan_bwd(const void* x, int64_t sxb, int64_t sxt, const void* dt, int64_t sdb, int64_t sdt, const float* A,
+                      const void* Bm, int64_t sbb, int64_t sbt, const void* Cm, int64_t scb, int64_t sct, const float* D,
+                      const void* z, int64_t szb, int64_t szt, const float* dt_bias, const int* lengths, const void* v,
+                      const float* states, const void* dy, int64_t syb, int64_t syt, const float* dstate_out, void* dx,
+                      void* ddt, float* dA, void* dB, void* dC, float* dD, void* dz, float* ddt_bias, float* dstate0,
+                      void* workspace, int64_t workspace_bytes, int dtype, int B, int T, int H, int P, int G, int N,
+                      void* stream);
+int rvit_ssm_scan_step(const void* x, int64_t sxb, const void* dt, int64_t sdb, const float* A, const void* Bm, int64_t sbb,
+                       const void* Cm, int64_t scb, const float* D, const void* z, int64_t szb, const float* dt_bias,
+                       float* state, void* y, int dtype, int B, int H, int P, int G, int N, void* stream);
+
+/* Norm behind a block, gate, residual scale and the norm before the next block in one pass:
+ *   h = residual + scale * gate o norm_post(y),  n = norm_pre(h);  norm = LayerNorm, or RMS (rms != 0; biases null then).
+ * residual, h: res_dtype [rows,E]; y, n: dtype [rows,E]; all packed, E <= 4096; weights and biases fp32 [E] (biases may be
+ * null).  gate_kind 0: none, 1: [E], 2: [rows / T, E] (one per sample of T rows), 3: [rows,E]; gate_dtype fp32 or dtype.
+ * stats fp32 [rows,4] (mean, 1/std of y, of h): written by fwd when not null, read by bwd. */
+int rvit_sandwich_norm_fwd(const void* residual, int res_dtype, const void* y, int dtype, const void* gate, int gate_kind,
+                           int gate_dtype, float scale, const float* post_w, const float* post_b, const float* pre_w,
+                           const float* pre_b, float eps, int rms, void* h, void* n, float* stats, int64_t rows, int T, int E,
+                           void* stream);
+int rvit_sandwich_norm_bwd_workspace(int64_t* bytes, int64_t rows, int T, int E, int gate_kind);
+int rvit_sandwich_norm_bwd(const void* residual, int res_dtype, const void* y, int dtype, const void* gate, int gate_kind,
+                           int gate_dtype, float scale, const float* post_w, const float* post_b, const float* pre_w,
+                           const float* pre_b, float eps, int rms, const float* stats, const void* dh, const void* dn,
+                           void* dresidual, void* dy, void* dgate, float* dpost_w, float* dpost_b, float* dpre_w,
+                           float* dpre_b, void* workspace, int64_t workspace_bytes, int64_t rows, int T, int E, void* stream);
 
 #ifdef __cplusplus
 }

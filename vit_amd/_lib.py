@@ -20,7 +20,7 @@ LIB_PATH = os.path.join(_HERE, "librvit.so")
 RVIT_BF16, RVIT_F32 = 0, 1
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_HSWISH, ACT_HSIGMOID = 0, 1, 2, 3, 4
 GATE_NONE, GATE_GELU_GRAD, GATE_RELU_MASK = 0, 1, 2
-ABI_VERSION = 29
+ABI_VERSION = 30
 DROP_PRE_RESIDUAL, DROP_POST_ACT = 1, 2
 
 
@@ -110,6 +110,20 @@ SIGNATURES = {
     "rvit_bn_bwd_reduce_pool": ([P, P, P, P, P, I, I, I, I, F, P, P, P], c_int),
     "rvit_bn_bwd_apply_pool": ([P, P, P, P, P, P, P, P, P, P, I, I, I, I, F, P], c_int),
     "rvit_maxpool3x3s2_bwd_nhwc": ([P, P, P, I, I, I, I, P], c_int),
+    "rvit_ssm_conv_fwd": ([P, L, L, P, P, P, P, P, P, I, I, I, I, I, I, P], c_int),
+    "rvit_ssm_conv_bwd_workspace": ([P, I, I, I, I], c_int),
+    "rvit_ssm_conv_bwd": ([P, L, L, P, P, P, P, P, L, L, P, P, P, P, P, P, L, I, I, I, I, I, I, P], c_int),
+    "rvit_ssm_conv_step": ([P, L, P, P, P, P, I, I, I, I, I, P], c_int),
+    "rvit_ssm_scan_plan": ([P, P, P, I, I, I, I, I, I], c_int),
+    "rvit_ssm_scan_fwd": ([P, L, L, P, L, L, P, P, L, L, P, L, L, P, P, L, L, P, P, P, P, P, P, P, P, L, I, I, I,
+                           I, I, I, I, P], c_int),
+    "rvit_ssm_scan_bwd": ([P, L, L, P, L, L, P, P, L, L, P, L, L, P, P, L, L, P, P, P, P, P, L, L, P, P, P, P, P,
+                           P, P, P, P, P, P, L, I, I, I, I, I, I, I, P], c_int),
+    "rvit_ssm_scan_step": ([P, L, P, L, P, P, L, P, L, P, P, L, P, P, P, I, I, I, I, I, I, P], c_int),
+    "rvit_sandwich_norm_fwd": ([P, I, P, I, P, I, I, F, P, P, P, P, F, I, P, P, P, L, I, I, P], c_int),
+    "rvit_sandwich_norm_bwd_workspace": ([P, L, I, I, I], c_int),
+    "rvit_sandwich_norm_bwd": ([P, I, P, I, P, I, I, F, P, P, P, P, F, I, P, P, P, P, P, P, P, P, P, P, P, L, L, I,
+                                I, P], c_int),
 }
 
 _lib = None

@@ -1,0 +1,256 @@
+// Short causal convolution per channel over the tokens of a sequence (the window in front of the selective scan), forward,
+// backward and the single-token form:   u[t] = bias + sum_k w[k] x[t - K + 1 + k],  y = u or silu(u).
+// HBM bound: a thread owns V channels (one 16-byte access) of a strip of tokens and slides its window through registers, so
+// x is read once but for K - 1 tokens between strips (which the caches hold), and a wave reads 1 KB of a token's row.
+#include "ssm_common.h"
+#include "rvit_internal.h"
+#include "ssm_args.h"
+
+namespace {
+
+template <typename T, int V>
+__device__ __forceinline__ void ldv(const T* p, float (&v)[V]) {
+  if constexpr (V == 1) v[0] = ssm_ld(p);
+  else if constexpr (V == 4) ssm_ld4(p, v);
+  else {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    v[0] = bf16_lo(u.x); v[1] = bf16_hi(u.x); v[2] = bf16_lo(u.y); v[3] = bf16_hi(u.y);
+    v[4] = bf16_lo(u.z); v[5] = bf16_hi(u.z); v[6] = bf16_lo(u.w); v[7] = bf16_hi(u.w);
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void stv(T* p, const float (&v)[V]) {
+  if constexpr (V == 1) ssm_st(p, v[0]);
+  else if constexpr (V == 4) ssm_st4(p, v);
+  else *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+template <int V> __device__ __forceinline__ void zero(float (&v)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = 0.f;
+}
+// token t of the sequence with the kept inputs before it: t >= -(K - 1); zero where neither has it
+template <typename T, int V, int K>
+__device__ __forceinline__ void ldx(const SsmConvArgs& a, int b, int t, int c0, int len, float (&v)[V]) {
+  if (t >= len) zero<V>(v);
+  else if (t >= 0) ldv<T, V>((const T*)a.x + b * a.sxb + t * a.sxt + c0, v);
+  else if (a.state && t >= 1 - K) ldv<T, V>((const T*)a.state + ((long)b * (K - 1) + (t + K - 1)) * a.C + c0, v);
+  else zero<V>(v);
+}
+template <int V, int K>
+__device__ __forceinline__ void ldw(const SsmConvArgs& a, int c0, float (&w)[K][V], float (&bias)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) w[k][j] = a.w[(long)(c0 + j) * K + k];
+    bias[j] = a.bias ? a.bias[c0 + j] : 0.f;
+  }
+}
+
+template <typename T, int V, int K>
+__global__ __launch_bounds__(256) void ssm_conv_fwd_kernel(SsmConvArgs a) {
+  const int groups = a.C / V;
+  const long id = (long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= (long)a.B * a.strips * groups) return;
+  const int c0 = (int)(id % groups) * V;
+  const long r = id / groups;
+  const int s = r % a.strips, b = r / a.strips;
+  const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+  const int t0 = s * a.strip, t1 = min(a.T, t0 + a.strip);
+  T* y = (T*)a.y + (long)b * a.T * a.C + c0;
+  float w[K][V], bias[V], win[K][V];
+  ldw<V, K>(a, c0, w, bias);
+#pragma unroll
+  for (int k = 0; k < K - 1; ++k) ldx<T, V, K>(a, b, t0 - (K - 1) + k, c0, len, win[k]);
+  for (int t = t0; t < t1; ++t) {
+    ldx<T, V, K>(a, b, t, c0, len, win[K - 1]);
+    float u[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      u[j] = bias[j];
+#pragma unroll
+      for (int k = 0; k < K; ++k) u[j] = fmaf(w[k][j], win[k][j], u[j]);
+      if (a.silu) u[j] *= ssm_sigmoid(u[j]);
+      if (t >= len) u[j] = 0.f;
+#pragma unroll
+      for (int k = 0; k + 1 < K; ++k) win[k][j] = win[k + 1][j];
+    }
+    stv<T, V>(y + (long)t * a.C, u);
+  }
+  if (a.state_out && s == 0) {       // the last K - 1 inputs before the sequence's end
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) {
+      float v[V];
+      ldx<T, V, K>(a, b, len - (K - 1) + k, c0, len, v);
+      stv<T, V>((T*)a.state_out + ((long)b * (K - 1) + k) * a.C + c0, v);
+    }
+  }
+}
+
+// du[t] = dy silu'(u), u recomputed; dx[t] = sum_k w[k] du[t + K - 1 - k]; dw[k] = sum_t du[t] x[t - K + 1 + k]; db = sum du.
+// A workgroup is 32 channel groups wide and 8 strips deep; its strips' dw, db are added in LDS in a fixed order and
+// written as one part, which ssm_conv_sum_kernel adds.
+template <typename T, int V, int K>
+__global__ __launch_bounds__(256) void ssm_conv_bwd_kernel(SsmConvArgs a) {
+  __shared__ float red[8][32][V];
+  const int groups = a.C / V;
+  const int gx = threadIdx.x & 31, sy = threadIdx.x >> 5;
+  const int cg = blockIdx.x * 32 + gx;
+  const int sblocks = (a.strips + 7) / 8;
+  const int b = blockIdx.y / sblocks, s = (blockIdx.y % sblocks) * 8 + sy;
+  float dw[K][V], db[V];
+#pragma unroll
+  for (int k = 0; k < K; ++k) zero<V>(dw[k]);
+  zero<V>(db);
+  if (cg < groups && s < a.strips) {
+    const int c0 = cg * V;
+    const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+    const int t0 = s * a.strip, t1 = min(a.T, t0 + a.strip);
+    T* dx = (T*)a.dx + (long)b * a.T * a.C + c0;
+    const T* dy = (const T*)a.dy + b * a.syb + c0;
+    const T* dso = a.dstate_out ? (const T*)a.dstate_out + (long)b * (K - 1) * a.C + c0 : nullptr;
+    float w[K][V], bias[V], win[K][V], du[K][V];
+    ldw<V, K>(a, c0, w, bias);
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) ldx<T, V, K>(a, b, t0 - (K - 1) + k, c0, len, win[k]);
+#pragma unroll
+    for (int k = 0; k < K; ++k) zero<V>(du[k]);
+    // token t enters: its du; then dx of token t - K + 1 is complete.  Tokens before the strip belong to the strip before
+    // (the first strip gives them to the kept inputs).
+    for (int t = t0; t < t1 + K - 1; ++t) {
+      ldx<T, V, K>(a, b, t, c0, len, win[K - 1]);
+      float g[V];
+      if (t < len) ldv<T, V>(dy + t * a.syt, g);
+      else zero<V>(g);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if (a.silu) {
+          float u = bias[j];
+#pragma unroll
+          for (int k = 0; k < K; ++k) u = fmaf(w[k][j], win[k][j], u);
+          const float sg = ssm_sigmoid(u);
+          g[j] *= sg + u * sg * (1.f - sg);
+          if (t >= len) g[j] = 0.f;
+        }
+        du[K - 1][j] = g[j];
+        if (t < t1) {
+          db[j] += g[j];
+#pragma unroll
+          for (int k = 0; k < K; ++k) dw[k][j] = fmaf(g[j], win[k][j], dw[k][j]);
+        }
+      }
+      const int to = t - (K - 1);
+      float o[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        o[j] = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) o[j] = fmaf(w[k][j], du[K - 1 - k][j], o[j]);
+      }
+      // du[i] holds token t - (K - 1) + i, so o is dx of token `to`: complete for to >= t0, and for the kept inputs
+      if (to >= t0 || s == 0) {
+        if (dso && to >= len - (K - 1) && to < len) {
+          float v[V];
+          ldv<T, V>(dso + (long)(to - len + K - 1) * a.C, v);
+#pragma unroll
+          for (int j = 0; j < V; ++j) o[j] += v[j];
+        }
+        if (to >= 0) stv<T, V>(dx + (long)to * a.C, o);
+        else if (a.dstate) stv<T, V>((T*)a.dstate + ((long)b * (K - 1) + to + K - 1) * a.C + c0, o);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+#pragma unroll
+        for (int k = 0; k + 1 < K; ++k) { win[k][j] = win[k + 1][j]; du[k][j] = du[k + 1][j]; }
+      }
+    }
+  }
+  // [part][K + 1][C]
+  float* part = a.part + (long)blockIdx.y * (K + 1) * a.C;
+#pragma unroll
+  for (int k = 0; k <= K; ++k) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < V; ++j) red[sy][gx][j] = k < K ? dw[k < K ? k : 0][j] : db[j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * V; i += 256) {
+      float v = 0.f;
+#pragma unroll
+      for (int y = 0; y < 8; ++y) v += red[y][i / V][i % V];
+      const int c = blockIdx.x * 32 * V + i;
+      if (c < a.C) part[(long)k * a.C + c] = v;
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void ssm_conv_sum_kernel(const float* part, float* dw, float* db, int parts, int C, int K) {
+  const long n = (long)(K + 1) * C, i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  double v = 0.0;
+  for (int p = 0; p < parts; ++p) v += (double)part[p * n + i];
+  const int k = i / C, c = i - (long)k * C;
+  if (k < K) dw[(long)c * K + k] = (float)v;
+  else if (db) db[c] = (float)v;
+}
+
+// one token: the kept inputs move by one, in place (a thread owns its channels of them)
+template <typename T, int V, int K>
+__global__ __launch_bounds__(256) void ssm_conv_step_kernel(SsmConvArgs a) {
+  const int groups = a.C / V;
+  const long id = (long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= (long)a.B * groups) return;
+  const int c0 = (int)(id % groups) * V, b = id / groups;
+  T* st = (T*)a.state_out + (long)b * (K - 1) * a.C + c0;
+  float w[K][V], bias[V], win[K][V];
+#pragma unroll
+  for (int k = 0; k < K - 1; ++k) ldv<T, V>(st + (long)k * a.C, win[k]);
+  ldv<T, V>((const T*)a.x + b * a.sxb + c0, win[K - 1]);
+  ldw<V, K>(a, c0, w, bias);
+  float u[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    u[j] = bias[j];
+#pragma unroll
+    for (int k = 0; k < K; ++k) u[j] = fmaf(w[k][j], win[k][j], u[j]);
+    if (a.silu) u[j] *= ssm_sigmoid(u[j]);
+  }
+#pragma unroll
+  for (int k = 0; k < K - 1; ++k) stv<T, V>(st + (long)k * a.C, win[k + 1]);
+  stv<T, V>((T*)a.y + (long)b * a.C + c0, u);
+}
+
+
+template <typename T, int V, int K>
+int launch(const SsmConvArgs& a, int what, hipStream_t st) {
+  const int groups = a.C / V;
+  if (what == SSM_CONV_BWD) {
+    const int sblocks = (a.strips + 7) / 8;
+    hipLaunchKernelGGL((ssm_conv_bwd_kernel<T, V, K>), dim3((groups + 31) / 32, a.B * sblocks), dim3(256), 0, st, a);
+    RVIT_CHECK_LAUNCH("ssm_conv_bwd");
+    hipLaunchKernelGGL(ssm_conv_sum_kernel, dim3((unsigned)(((long)(K + 1) * a.C + 255) / 256)), dim3(256), 0, st, a.part, a.dw, a.dbias, a.B * sblocks, a.C, K);
+    RVIT_CHECK_LAUNCH("ssm_conv_sum");
+    return RVIT_OK;
+  }
+  const long n = (long)a.B * (what == SSM_CONV_FWD ? a.strips : 1) * groups;
+  const dim3 grid((unsigned)((n + 255) / 256));
+  if (what == SSM_CONV_FWD) hipLaunchKernelGGL((ssm_conv_fwd_kernel<T, V, K>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((ssm_conv_step_kernel<T, V, K>), grid, dim3(256), 0, st, a);
+  RVIT_CHECK_LAUNCH("ssm_conv");
+  return RVIT_OK;
+}
+template <typename T, int V>
+int launch_k(const SsmConvArgs& a, int what, hipStream_t st) {
+  switch (a.K) {
+    case 2: return launch<T, V, 2>(a, what, st);
+    case 3: return launch<T, V, 3>(a, what, st);
+    case 4: return launch<T, V, 4>(a, what, st);
+    case 5: return launch<T, V, 5>(a, what, st);
+    default: return launch<T, V, 6>(a, what, st);
+  }
+}
+
+}  // namespace
+
+int rvit_ssm_conv_impl(const SsmConvArgs& a, int dtype, int what, hipStream_t st) {
+  if (dtype == RVIT_BF16) return a.vec ? launch_k<bf16, 8>(a, what, st) : launch_k<bf16, 1>(a, what, st);
+  return a.vec ? launch_k<float, 4>(a, what, st) : launch_k<float, 1>(a, what, st);
+}
