@@ -137,3 +137,24 @@ def test_c_entries_refuse_without_a_launch():
     assert lib.rvit_ssm_scan_fwd(*scan, None, 0, 2, 1, 64, 1, 64, 1, 64, None) == -1     # dtype
     assert lib.rvit_ssm_conv_fwd(64, 1, 1, 64, None, 128, None, 64, 128, 1, 1, 8, 8, 4, 0, None) == -1   # the kept inputs in place
     assert lib.rvit_sandwich_norm_fwd(64, 1, 64, 1, 64, 4, 1, 1.0, 64, None, 64, None, 1e-5, 0, 64, 64, None, 4, 2, 8, None) == -1
+
+
+def test_temporal_encoder_refusals():
+    from vit_amd.sequence import CNNViTSequence, TemporalEncoder
+    with pytest.raises(ValueError, match="causal"):
+        TemporalEncoder(128, 64, model_type="ssm")                                     # bidirectional by default
+    with pytest.raises(NotImplementedError):
+        TemporalEncoder(128, 40, bidirectional=False, model_type="ssm")
+    with pytest.raises(NotImplementedError):
+        TemporalEncoder(130, 64, bidirectional=False, model_type="ssm")
+    enc = TemporalEncoder(128, 64, 2, bidirectional=False, model_type="ssm")
+    assert enc.output_dim == 64
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        enc(torch.zeros(1, 4, 128))
+    cfg = dict(backbone="patch16", embed_dim=128, num_heads=2, num_layers=1, dropout=0.0, temporal_hidden=64, temporal_layers=1)
+    with pytest.raises(ValueError, match="keeps no state"):
+        CNNViTSequence(11, cfg).forward_temporal_step(torch.zeros(1, 128))
+    m = CNNViTSequence(11, dict(cfg, temporal_model="ssm"))
+    assert not m.temporal_encoder.bidirectional and m.classifier["0"].weight.shape == (32, 64)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        m.forward_temporal_step(torch.zeros(1, 128))

@@ -10,7 +10,9 @@ loads unchanged.  Arithmetic:
     parameters), the step's backward likewise; weight / bias / input gradients from the saved gate gradients
     with the package's GEMM kernels;
   * classifier: the same fused GEMM epilogues as the single-frame head.
-Both `model_type='lstm'` (the reference default, train_vit.py:267) and 'gru' are built.
+Both `model_type='lstm'` (the reference default, train_vit.py:267) and 'gru' are built.  `model_type='ssm'` is this package's
+own third form: a stack of state-space layers (vit_amd/ssm.py), which trains over the frames of a window in parallel and, in
+streaming, goes on from a kept state of fixed size, one frame at a time, instead of running the window again.
 There is no CPU path.
 """
 from __future__ import annotations
@@ -25,7 +27,7 @@ import numpy as np
 import torch
 import torch.nn as nn
 
-from . import _lib, ops
+from . import _lib, ops, ssm
 from .model import CNNViTHybrid, _Linear
 from .ops import _ptr, _stream, check
 
@@ -57,13 +59,198 @@ class _LSTMParams(nn.Module):
         return tuple(getattr(self, f"{n}_l{layer}{s}") for n in ("weight_ih", "weight_hh", "bias_ih", "bias_hh"))
 
 
+class _Linear16(torch.autograd.Function):
+    """y = x @ w.T (+ bias) on bf16 operands (fp32 accumulation, bf16 result): x [rows,K] bf16, w fp32 [N,K]."""
+
+    @staticmethod
+    def forward(ctx, x, w, bias):
+        N, K = w.shape
+        Np = 8 * ((N + 7) // 8)                 # the weight-gradient kernel takes whole groups of 8 rows
+        w16 = w.detach().to(BF16)
+        if Np != N:
+            w16 = torch.cat([w16, w16.new_zeros(Np - N, K)])
+        y = torch.empty(x.shape[0], Np, dtype=BF16, device=x.device)
+        b = bias if bias is None or Np == N else torch.cat([bias.detach(), bias.new_zeros(Np - N)])
+        ops.gemm(x, w16, y, bias=None if b is None else b.detach())
+        ctx.save_for_backward(x, w16)
+        ctx.n, ctx.has_bias = N, bias is not None
+        return y if Np == N else y[:, :N]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w16 = ctx.saved_tensors
+        N, (Np, K) = ctx.n, w16.shape
+        with torch.cuda.device(x.device):
+            if Np != N:
+                dyp = dy.new_zeros(dy.shape[0], Np)
+                dyp[:, :N] = dy
+                dy = dyp
+            dy = dy.contiguous()
+            dx = torch.empty_like(x)
+            ops.gemm(dy, w16.t().contiguous(), dx)
+            dw = torch.zeros(N, K, dtype=F32, device=x.device)
+            ops.wgrad(dy, x, dw, n_store=N)
+            db = None
+            if ctx.has_bias:
+                db = torch.zeros(Np, dtype=F32, device=x.device)
+                ops.colsum(dy, db)
+                db = db[:N].contiguous()
+        return dx, dw, db
+
+
+class _Norm16(torch.autograd.Function):
+    """LayerNorm of fp32 rows to bf16 (the norm before the first layer, which has no block in front of it)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        rows = x.shape[0]
+        y = torch.empty(x.shape, dtype=BF16, device=x.device)
+        mean, rstd = (torch.empty(rows, dtype=F32, device=x.device) for _ in range(2))
+        ops.layernorm(x, weight.detach(), bias.detach(), y, mean=mean, rstd=rstd)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        with torch.cuda.device(x.device):
+            dx = torch.empty_like(x)
+            dw, db = torch.zeros_like(weight), torch.zeros_like(weight)
+            ops.layernorm_bwd(dy.contiguous(), x, mean, rstd, weight, dx, dw, db, accumulate=False)
+        return dx, dw, db
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, seed):
+        ctx.p, ctx.seed = p, seed
+        return ops.dropout_apply(x, torch.empty_like(x), p, seed)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        with torch.cuda.device(dy.device):
+            dy = dy.contiguous()
+            return ops.dropout_apply(dy, torch.empty_like(dy), ctx.p, ctx.seed), None, None
+
+
+class SSMStack(nn.Module):
+    """Layers of n -> in_proj -> short causal convolution (SiLU) of x, B, C -> selective scan, gated -> out_proj, each followed
+    by the norm behind it, its gate, the residual connection and the norm before the next in one pass (ssm.sandwich_norm).
+    Inner width 2 x hidden in heads of 64 channels, one group of B and C.  The residual stream is fp32, activations bf16,
+    parameters fp32."""
+
+    HEAD, WINDOW = 64, 4
+
+    def __init__(self, input_dim: int, hidden: int, num_layers: int, states: int = 64):
+        super().__init__()
+        self.input_size, self.hidden_size, self.num_layers, self.states = input_dim, hidden, num_layers, states
+        self.inner = 2 * hidden
+        self.heads = self.inner // self.HEAD
+        self.conv_width = self.inner + 2 * states
+        self.proj_width = self.conv_width + self.inner + self.heads
+        lin = lambda fout, fin: torch.empty(fout, fin).uniform_(-1 / math.sqrt(fin), 1 / math.sqrt(fin))  # noqa: E731
+        reg = lambda n, v: self.register_parameter(n, nn.Parameter(v))  # noqa: E731
+        reg("weight_embed", lin(hidden, input_dim))
+        reg("bias_embed", torch.zeros(hidden))
+        for k in range(num_layers + 1):          # norm k stands before layer k; the last one ends the stack
+            reg(f"pre_weight_l{k}", torch.ones(hidden))
+            reg(f"pre_bias_l{k}", torch.zeros(hidden))
+        for k in range(num_layers):
+            reg(f"in_proj_l{k}", lin(self.proj_width, hidden))
+            reg(f"conv_weight_l{k}", torch.empty(self.conv_width, self.WINDOW).uniform_(-0.5, 0.5))
+            reg(f"conv_bias_l{k}", torch.zeros(self.conv_width))
+            reg(f"A_log_l{k}", torch.empty(self.heads).uniform_(0.0, math.log(16.0)))
+            reg(f"D_l{k}", torch.ones(self.heads))
+            d = torch.exp(torch.empty(self.heads).uniform_(math.log(1e-3), math.log(1e-1)))
+            reg(f"dt_bias_l{k}", d + torch.log(-torch.expm1(-d)))       # softplus of it is d
+            reg(f"out_proj_l{k}", lin(hidden, self.inner))
+            reg(f"post_weight_l{k}", torch.ones(hidden))
+            reg(f"post_bias_l{k}", torch.zeros(hidden))
+            reg(f"gate_l{k}", torch.full((hidden,), 0.5))
+
+    def _p(self, name: str, k: int) -> torch.Tensor:
+        return getattr(self, f"{name}_l{k}")
+
+    def _split(self, u: torch.Tensor):
+        x, Bm, Cm = torch.split(u, [self.inner, self.states, self.states], dim=-1)
+        return x.unflatten(-1, (self.heads, self.HEAD)), Bm.unsqueeze(-2), Cm.unsqueeze(-2)
+
+    def _start(self, x2d: torch.Tensor):
+        h = _Linear16.apply(x2d.to(BF16), self.weight_embed, self.bias_embed).float()
+        return h, _Norm16.apply(h, self.pre_weight_l0, self.pre_bias_l0)
+
+    def _join(self, k: int, h, y):
+        return ssm.sandwich_norm(h, y, self._p("post_weight", k), self._p("post_bias", k), self._p("pre_weight", k + 1),
+                                 self._p("pre_bias", k + 1), gate=self._p("gate", k))
+
+    def run(self, x: torch.Tensor, lengths=None, p_drop: float = 0.0, base_seed: int = 0, cache=None) -> torch.Tensor:
+        """x [B,T,input] -> the normalised stream [B,T,hidden] bf16.  `cache` (a list): goes on from it, and leaves the states
+        behind each sample's last frame in it."""
+        B, T, _ = x.shape
+        h, n = self._start(x.reshape(B * T, -1))
+        h, n = h.view(B, T, -1), n.view(B, T, -1)
+        widths = [self.conv_width, self.inner, self.heads]
+        before, behind = list(cache) if cache else [(None, None)] * self.num_layers, []
+        for k in range(self.num_layers):
+            proj = _Linear16.apply(n.reshape(B * T, -1), self._p("in_proj", k), None).view(B, T, -1)
+            xbc, z, dt = torch.split(proj, widths, dim=-1)
+            conv0, scan0 = before[k]
+            u, conv1 = ssm.causal_conv(xbc, self._p("conv_weight", k), self._p("conv_bias", k), activation="silu", state=conv0,
+                                       lengths=lengths, return_state=True)
+            xs, Bm, Cm = self._split(u)
+            y, scan1 = ssm.selective_scan(xs, dt, -torch.exp(self._p("A_log", k)), Bm, Cm, D=self._p("D", k),
+                                          z=z.unflatten(-1, (self.heads, self.HEAD)), dt_bias=self._p("dt_bias", k), state=scan0,
+                                          lengths=lengths, return_state=True)
+            behind.append((conv1, scan1))
+            o = _Linear16.apply(y.reshape(B * T, self.inner), self._p("out_proj", k), None)
+            if p_drop > 0.0 and k < self.num_layers - 1:     # as nn.LSTM: between layers only
+                o = _Dropout.apply(o, p_drop, _site_seed(base_seed, 100 + k))
+            h, n = self._join(k, h, o.view(B, T, -1))
+        if cache is not None:
+            cache[:] = behind
+        return n
+
+    def new_cache(self, B: int, device) -> list:
+        """The states before any frame."""
+        return [(torch.zeros(B, self.WINDOW - 1, self.conv_width, dtype=BF16, device=device),
+                 torch.zeros(B, self.heads, self.HEAD, self.states, dtype=F32, device=device)) for _ in range(self.num_layers)]
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, cache: list) -> torch.Tensor:
+        """One frame: x [B,input] -> [B,hidden] bf16; the cache's states advance in place."""
+        h, n = self._start(x)
+        widths = [self.conv_width, self.inner, self.heads]
+        for k in range(self.num_layers):
+            xbc, z, dt = torch.split(_Linear16.apply(n, self._p("in_proj", k), None), widths, dim=-1)
+            conv, scan = cache[k]
+            xs, Bm, Cm = self._split(ssm.causal_conv_step(xbc, self._p("conv_weight", k), self._p("conv_bias", k), conv, activation="silu"))
+            y = ssm.selective_scan_step(xs, dt, -torch.exp(self._p("A_log", k)), Bm, Cm, scan, D=self._p("D", k),
+                                        z=z.unflatten(-1, (self.heads, self.HEAD)), dt_bias=self._p("dt_bias", k))
+            h, n = self._join(k, h, _Linear16.apply(y.reshape(-1, self.inner), self._p("out_proj", k), None))
+        return n
+
+
 class TemporalEncoder(nn.Module):
-    """train_vit.py:188-229: (bi)LSTM over frame features; returns [forward h at t = T-1 | backward h at t = 0]."""
+    """train_vit.py:188-229: (bi)LSTM over frame features; returns [forward h at t = T-1 | backward h at t = 0].
+    model_type='ssm': a stack of state-space layers (causal: bidirectional=False); returns its output at t = T-1."""
 
     def __init__(self, input_dim, hidden_dim=256, num_layers=2, dropout=0.3, bidirectional=True, model_type="lstm"):
         super().__init__()
-        if model_type not in ("lstm", "gru"):
+        if model_type not in ("lstm", "gru", "ssm"):
             raise ValueError(f"Unknown model_type: {model_type}")
+        if model_type == "ssm":
+            if bidirectional:
+                raise ValueError("model_type='ssm' is causal: bidirectional=False")
+            if hidden_dim % 32 or input_dim % 8 or not 0 < hidden_dim <= 2048 or num_layers < 1:
+                raise NotImplementedError("the state-space layers need hidden_dim % 32 == 0 (at most 2048) and input_dim % 8 == 0")
+            self.model_type, self.bidirectional, self.hidden_dim, self.num_layers = model_type, False, hidden_dim, num_layers
+            self.dropout = float(dropout) if num_layers > 1 else 0.0
+            self.rnn = SSMStack(input_dim, hidden_dim, num_layers)
+            self.output_dim = hidden_dim
+            return
         if hidden_dim % 8 or input_dim % 4:
             raise NotImplementedError("the recurrent kernels need hidden_dim % 8 == 0 and input_dim % 4 == 0")
         self.model_type, self.bidirectional, self.hidden_dim = model_type, bidirectional, hidden_dim
@@ -73,7 +260,26 @@ class TemporalEncoder(nn.Module):
         self.output_dim = hidden_dim * (2 if bidirectional else 1)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.model_type == "ssm":
+            return self.ssm_features(x)[0]
         return _TemporalFunction.apply(x, self, None, self.training and torch.is_grad_enabled(), *self.parameters())
+
+    def ssm_features(self, x: torch.Tensor, lengths: Optional[torch.Tensor] = None, cache: Optional[list] = None):
+        """-> (feature [B,hidden] fp32 of each sample's last frame, seed of this pass's dropout sites)."""
+        if not x.is_cuda:
+            raise RuntimeError("the temporal encoder runs on the GPU through librvit only; there is no CPU fallback")
+        if x.dim() != 3 or x.shape[2] != self.rnn.input_size or x.shape[0] < 1 or x.shape[1] < 1:
+            raise ValueError(f"expected features [B,T,{self.rnn.input_size}], got {tuple(x.shape)}")
+        train = self.training and torch.is_grad_enabled()
+        base = int(torch.randint(0, 2 ** 62, (1,)).item()) if train else 0
+        with torch.cuda.device(x.device):
+            n = self.rnn.run(x, lengths, self.dropout if train else 0.0, base, cache)
+            if lengths is None:
+                last = n[:, -1]
+            else:
+                at = (lengths.long().clamp(1, x.shape[1]) - 1)[:, None, None].expand(-1, 1, n.shape[2])
+                last = n.gather(1, at)[:, 0]
+            return last.float(), base
 
 
 def _site_seed(base: int, site: int) -> int:
@@ -204,6 +410,69 @@ def _scatter_last(enc: TemporalEncoder, dtf: torch.Tensor, B: int, T: int) -> to
     return dtop
 
 
+def _cls_forward(cls, tf: torch.Tensor, train: bool, base: int):
+    """temporal feature fp32 [B,D] -> (logits fp32 [B,classes], what the backward needs)."""
+    B, D = tf.shape
+    l0, l3 = cls["0"], cls["3"]
+    C = l3.weight.shape[0]
+    tf16 = tf.to(BF16)
+    h = torch.empty(B, D // 2, dtype=BF16, device=tf.device)
+    u0 = torch.empty(B, D // 2, dtype=BF16, device=tf.device) if train else None
+    p = cls.drop_p if train else 0.0
+    seed = _site_seed(base, 1) if p > 0 else 0
+    ops.gemm(tf16, l0.weight.detach().to(BF16), h, bias=l0.bias.detach(), act="gelu", preact=u0,
+             drop=("post_act", p, seed) if p > 0 else None)
+    logits = torch.empty(B, C, dtype=F32, device=tf.device)
+    ops.gemm(h, l3.weight.detach().to(BF16), logits, bias=l3.bias.detach())
+    return logits, (tf16, h, u0, p, seed)
+
+
+def _cls_backward(cls, saved, dout: torch.Tensor):
+    """-> (gradient of the temporal feature, [gradients of the classifier's parameters])."""
+    tf16, h, u0, p, seed = saved
+    B, dev = tf16.shape[0], dout.device
+    l0, l3 = cls["0"], cls["3"]
+    C, Dh = l3.weight.shape
+    Cp = 16 * ((C + 15) // 16)
+    dl16 = torch.zeros(B, Cp, dtype=BF16, device=dev)
+    dl16[:, :C] = dout
+    g3 = torch.zeros(C, Dh, dtype=F32, device=dev)
+    ops.wgrad(dl16, h, g3, n_store=C)
+    b3 = torch.zeros(Cp, dtype=F32, device=dev)
+    ops.colsum(dl16, b3)
+    w3t = torch.zeros(Dh, Cp, dtype=BF16, device=dev)
+    w3t[:, :C] = l3.weight.detach().t().to(BF16)
+    dh = torch.empty(B, Dh, dtype=BF16, device=dev)
+    ops.gemm(dl16, w3t, dh, gate=u0, gate_mode="gelu_grad", drop=("post_act", p, seed) if p > 0 else None)
+    g0 = torch.zeros(Dh, tf16.shape[1], dtype=F32, device=dev)
+    ops.wgrad(dh, tf16, g0)
+    b0 = torch.zeros(Dh, dtype=F32, device=dev)
+    ops.colsum(dh, b0)
+    dtf = torch.empty(B, tf16.shape[1], dtype=F32, device=dev)
+    ops.gemm(dh, l0.weight.detach().t().contiguous().to(BF16), dtf)
+    return dtf, [g0, b0, g3, b3[:C].contiguous()]
+
+
+class _ClassifierFunction(torch.autograd.Function):
+    """temporal feature [B,D] -> logits, behind an encoder whose own backward is autograd's (model_type='ssm')."""
+
+    @staticmethod
+    def forward(ctx, tf, cls, train: bool, base: int, *params):
+        with torch.cuda.device(tf.device):
+            logits, ctx.cls_saved = _cls_forward(cls, tf.detach(), train, base)
+        ctx.cls, ctx.trained = cls, train
+        return logits
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        if not ctx.trained:
+            raise RuntimeError("backward through a forward that ran in eval mode / without grad")
+        with torch.cuda.device(dout.device):
+            dtf, grads = _cls_backward(ctx.cls, ctx.cls_saved, dout)
+        return (dtf, None, None, None, *grads)
+
+
 class _TemporalFunction(torch.autograd.Function):
     """features [B,T,E] -> temporal feature [B,out_dim] (classifier=None) or logits [B,classes]."""
 
@@ -224,20 +493,7 @@ class _TemporalFunction(torch.autograd.Function):
         ctx.enc, ctx.cls, ctx.saved, ctx.shape = enc, cls, saved, tuple(feats.shape)
         if cls is None:
             return tf
-        D = enc.output_dim
-        B = tf.shape[0]
-        l0, l3 = cls["0"], cls["3"]
-        C = l3.weight.shape[0]
-        tf16 = tf.to(BF16)
-        h = torch.empty(B, D // 2, dtype=BF16, device=tf.device)
-        u0 = torch.empty(B, D // 2, dtype=BF16, device=tf.device) if train else None
-        p = cls.drop_p if train else 0.0
-        ctx.cls_seed = _site_seed(base, 1) if p > 0 else 0
-        ops.gemm(tf16, l0.weight.detach().to(BF16), h, bias=l0.bias.detach(), act="gelu", preact=u0,
-                 drop=("post_act", p, ctx.cls_seed) if p > 0 else None)
-        logits = torch.empty(B, C, dtype=F32, device=tf.device)
-        ops.gemm(h, l3.weight.detach().to(BF16), logits, bias=l3.bias.detach())
-        ctx.cls_saved = (tf16, h, u0, p)
+        logits, ctx.cls_saved = _cls_forward(cls, tf, train, base)
         return logits
 
     @staticmethod
@@ -256,27 +512,7 @@ class _TemporalFunction(torch.autograd.Function):
         if cls is None:
             dtf = dout.contiguous().float()
         else:
-            tf16, h, u0, p = ctx.cls_saved
-            l0, l3 = cls["0"], cls["3"]
-            C, Dh = l3.weight.shape
-            Cp = 16 * ((C + 15) // 16)
-            dl16 = torch.zeros(B, Cp, dtype=BF16, device=dev)
-            dl16[:, :C] = dout
-            g3 = torch.zeros(C, Dh, dtype=F32, device=dev)
-            ops.wgrad(dl16, h, g3, n_store=C)
-            b3 = torch.zeros(Cp, dtype=F32, device=dev)
-            ops.colsum(dl16, b3)
-            w3t = torch.zeros(Dh, Cp, dtype=BF16, device=dev)
-            w3t[:, :C] = l3.weight.detach().t().to(BF16)
-            dh = torch.empty(B, Dh, dtype=BF16, device=dev)
-            ops.gemm(dl16, w3t, dh, gate=u0, gate_mode="gelu_grad", drop=("post_act", p, ctx.cls_seed) if p > 0 else None)
-            g0 = torch.zeros(Dh, tf16.shape[1], dtype=F32, device=dev)
-            ops.wgrad(dh, tf16, g0)
-            b0 = torch.zeros(Dh, dtype=F32, device=dev)
-            ops.colsum(dh, b0)
-            dtf = torch.empty(B, tf16.shape[1], dtype=F32, device=dev)
-            ops.gemm(dh, l0.weight.detach().t().contiguous().to(BF16), dtf)
-            cls_grads = [g0, b0, g3, b3[:C].contiguous()]
+            dtf, cls_grads = _cls_backward(cls, ctx.cls_saved, dout)
         dfeats, g = _lstm_backward(enc, saved, _scatter_last(enc, dtf, B, T))
         enc_grads = [g[n] for n, _ in enc.rnn.named_parameters()]
         return (dfeats, None, None, None, *enc_grads, *cls_grads)
@@ -301,7 +537,7 @@ class CNNViTSequence(nn.Module):
         self.temporal_encoder = TemporalEncoder(input_dim=config["embed_dim"], hidden_dim=config.get("temporal_hidden", 256),
                                                 num_layers=config.get("temporal_layers", 2),
                                                 dropout=config.get("temporal_dropout", 0.3),
-                                                bidirectional=config.get("temporal_bidirectional", True),
+                                                bidirectional=config.get("temporal_bidirectional", config.get("temporal_model", "lstm") != "ssm"),
                                                 model_type=config.get("temporal_model", "lstm"))
         d = self.temporal_encoder.output_dim
         if (d // 2) % 8:
@@ -324,8 +560,29 @@ class CNNViTSequence(nn.Module):
     def forward_temporal_only(self, spatial_features):
         """[B,T,E] features -> logits (streaming)."""
         enc = self.temporal_encoder
+        if enc.model_type == "ssm":
+            tf, base = enc.ssm_features(spatial_features)
+            return _ClassifierFunction.apply(tf, self.classifier, self.training and torch.is_grad_enabled(), base,
+                                             *self.classifier.parameters())
         return _TemporalFunction.apply(spatial_features, enc, self.classifier, self.training and torch.is_grad_enabled(),
                                        *enc.parameters(), *self.classifier.parameters())
+
+    @torch.no_grad()
+    def forward_temporal_step(self, spatial_features, cache: Optional[list] = None):
+        """temporal_model='ssm': one frame's features [B,E] -> (logits, cache).  The cache (None: before any frame) holds every
+        layer's states and advances in place: the cost of a frame does not grow with the number of frames behind it."""
+        enc = self.temporal_encoder
+        if enc.model_type != "ssm":
+            raise ValueError(f"temporal_model={enc.model_type!r} keeps no state between frames: use forward_temporal_only on a window")
+        if not spatial_features.is_cuda:
+            raise RuntimeError("the temporal encoder runs on the GPU through librvit only; there is no CPU fallback")
+        if spatial_features.dim() != 2 or spatial_features.shape[1] != self.embed_dim:
+            raise ValueError(f"expected features [B,{self.embed_dim}], got {tuple(spatial_features.shape)}")
+        with torch.cuda.device(spatial_features.device):
+            if cache is None:
+                cache = enc.rnn.new_cache(spatial_features.shape[0], spatial_features.device)
+            tf = enc.rnn.step(spatial_features, cache).float()
+            return _cls_forward(self.classifier, tf, False, 0)[0], cache
 
     def freeze_backbone(self):
         for p in self.spatial_encoder.cnn_backbone.parameters():
@@ -352,9 +609,11 @@ class StreamingClassifier:
     weights_only=True) or a ready (model, classes, config) triple."""
 
     def __init__(self, model_path=None, device: str = "auto", smoothing_window: int = 3, *, model=None, classes=None,
-                 config=None, confidence_threshold: float = 0.5, device_preprocess: bool = False):
+                 config=None, confidence_threshold: float = 0.5, device_preprocess: bool = False, carry_state: bool = False):
         # device_preprocess: uint8 frames given as arrays are resized / normalised on the GPU (vit_amd.pipeline, the
         # same arithmetic as the host transform, bit for bit) instead of by Pillow on the host
+        # carry_state (temporal_model='ssm'): every frame goes on from the states the frames before it left, back to the last
+        # reset(), instead of running the last `sequence_length` frames again
         self.device_preprocess = bool(device_preprocess)
         self._pre = {}
         self.device = torch.device("cuda" if device == "auto" else device)
@@ -379,6 +638,10 @@ class StreamingClassifier:
         self.sequence_length = self.config.get("sequence_length", 8) if self.mode == "sequence" else 1
         self.confidence_threshold = confidence_threshold
         self.model = model.to(self.device).eval()
+        self.carry_state = bool(carry_state)
+        if self.carry_state and (self.mode != "sequence" or self.model.temporal_encoder.model_type != "ssm"):
+            raise ValueError("carry_state needs a sequence model with temporal_model='ssm'")
+        self._cache = None
         self.feature_buffer = deque(maxlen=self.sequence_length)
         self.prediction_history = deque(maxlen=smoothing_window)
         self.frame_count = 0
@@ -412,7 +675,11 @@ class StreamingClassifier:
         start = time.perf_counter()
         tensor = self._preprocess(frame).unsqueeze(0).to(self.device)
         self.frame_count += 1
-        if self.mode == "sequence":
+        if self.carry_state:
+            logits, self._cache = self.model.forward_temporal_step(self.model.forward_spatial_only(tensor).view(1, -1), self._cache)
+            if self.frame_count < self.sequence_length:
+                return None
+        elif self.mode == "sequence":
             self.feature_buffer.append(self.model.forward_spatial_only(tensor))
             if len(self.feature_buffer) < self.sequence_length:
                 return None
@@ -430,6 +697,7 @@ class StreamingClassifier:
                                 latency_ms=(time.perf_counter() - start) * 1000)
 
     def reset(self):
+        self._cache = None
         self.feature_buffer.clear()
         self.prediction_history.clear()
         self.frame_count = 0
