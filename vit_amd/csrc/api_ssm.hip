@@ -9,28 +9,28 @@ namespace {
 bool at(const void* p, unsigned a) { return (((uintptr_t)p) & (a - 1)) == 0; }
 int es(int dtype) { return dtype == RVIT_BF16 ? 2 : 4; }
 
-// Segments of a sequence.  One workgroup walks a (sample, head, 64 channels); with fewer than one of them per compute unit
-// the sequence is cut, at the price of a pass that only computes states.
+// Segments of a sequence.  One workgroup walks a (sample, head, 64 channels), and a compute unit holds two of them; where there
+// are too few to fill the chip the sequence is cut, at the price of a pass that only computes states.
 void segments(SsmScanArgs& a) {
   a.pblocks = (a.P + 63) / 64;
   a.nchunks = (a.T + SSM_CHUNK - 1) / SSM_CHUNK;
   const long rows = (long)a.B * a.H * a.pblocks;
-  long n = rows >= 256 ? 1 : (512 + rows - 1) / rows;
+  long n = rows >= 512 ? 1 : 512 / rows;
   if (n > a.nchunks / 4) n = a.nchunks / 4;
   if (n < 1) n = 1;
   a.seg_chunks = n == 1 ? a.nchunks : (int)((a.nchunks + n - 1) / n);
   a.nseg = a.seg_chunks ? (a.nchunks + a.seg_chunks - 1) / a.seg_chunks : 1;
   if (a.nseg < 1) a.nseg = 1;
-  a.seg_stride = (long)a.B * a.H * a.P * a.N;
+  a.seg_stride = (long)a.B * a.H * a.pblocks * 64 * ssm_padded_n(a.N);
 }
 int64_t seg_bytes(const SsmScanArgs& a) {
   return a.nseg > 1 ? (int64_t)a.nseg * (a.seg_stride * 4 + (int64_t)a.B * a.H * 8) + 16 : 0;
 }
-// Parts of a group's heads in the backward pass: one workgroup per (sample, chunk, group) where they fill the chip twice.
+// Parts of a group's heads in the backward pass: a compute unit holds one workgroup of its chunk kernel.
 void split_heads(SsmBwdArgs& a) {
   const int r = a.f.H / a.f.G;
   const long rows = (long)a.f.B * a.f.nchunks * a.f.G;
-  long n = rows >= 512 ? 1 : (512 + rows - 1) / (rows > 0 ? rows : 1);
+  long n = rows >= 256 || rows < 1 ? 1 : 256 / rows;
   if (n > r) n = r;
   a.hper = (int)((r + n - 1) / n);
   a.hsplit = (r + a.hper - 1) / a.hper;
@@ -55,7 +55,8 @@ int inputs(SsmScanArgs& a, int dtype, const void* x, int64_t sxb, int64_t sxt, c
   a.x = x; a.dt = dt; a.A = A; a.Bm = Bm; a.Cm = Cm; a.D = D; a.z = z; a.dt_bias = dt_bias; a.lengths = lengths;
   a.sxb = sxb; a.sxt = sxt; a.sdb = sdb; a.sdt = sdt; a.sbb = sbb; a.sbt = sbt; a.scb = scb; a.sct = sct; a.szb = szb; a.szt = szt;
   const int V = 16 / es(dtype);
-  a.vec_x = at(x, 16) && sxb % V == 0 && sxt % V == 0 && a.P % V == 0;
+  const int64_t most = 1 << 24;       // token strides that fit a 32-bit offset over the tokens of a chunk
+  a.vec_x = at(x, 16) && sxt < most && sbt < most && sct < most && sxb % V == 0 && sxt % V == 0 && a.P % V == 0;
   a.vec_bc = at(Bm, 16) && at(Cm, 16) && sbb % V == 0 && sbt % V == 0 && scb % V == 0 && sct % V == 0 && a.N % V == 0;
   a.vec_z = at(z, 4 * es(dtype)) && szb % 4 == 0 && szt % 4 == 0 && a.P % 4 == 0;
   return RVIT_OK;
@@ -98,7 +99,8 @@ int rvit_ssm_scan_fwd(const void* x, int64_t sxb, int64_t sxt, const void* dt, i
                  (long long)workspace_bytes, (long long)seg_bytes(a) + 16);
   a.state0 = state0; a.y = y; a.v = v; a.state_out = state_out; a.states = states;
   a.vec_y = at(y, 4 * es(dtype)) && at(v, 4 * es(dtype)) && P % 4 == 0;
-  a.vec_state = N % 4 == 0 && at(state0, 16) && at(state_out, 16) && at(states, 16);
+  a.vec_state = N % 4 == 0 && at(state0, 16) && at(state_out, 16);
+  RVIT_CHECK_ARG(at(states, 16), "ssm_scan_fwd: states alignment");
   char* ws = (char*)workspace;
   take_segments(a, ws);
   return rvit_ssm_scan_fwd_impl(a, dtype, (hipStream_t)stream);
@@ -123,7 +125,8 @@ int rvit_ssm_scan_bwd(const void* x, int64_t sxb, int64_t sxt, const void* dt, i
   a.dy = dy; a.syb = syb; a.syt = syt; a.dstate_out = dstate_out;
   a.dx = dx; a.dz = z ? dz : nullptr; a.ddt = ddt; a.dB = dB; a.dC = dC; a.dA = dA; a.dD = dD; a.dbias = ddt_bias; a.dstate0 = dstate0;
   a.f.vec_y = at(v, 4 * es(dtype)) && P % 4 == 0;
-  a.f.vec_state = N % 4 == 0 && at(states, 16) && at(dstate_out, 16) && at(dstate0, 16);
+  a.f.vec_state = N % 4 == 0 && at(dstate_out, 16) && at(dstate0, 16);
+  RVIT_CHECK_ARG(at(states, 16), "ssm_scan_bwd: states alignment");
   a.vec_dy = at(dy, 4 * es(dtype)) && syb % 4 == 0 && syt % 4 == 0 && P % 4 == 0;
   a.vec_out = at(dx, 4 * es(dtype)) && at(dz, 4 * es(dtype)) && P % 4 == 0;
   a.vec_dbc = at(dB, 4 * es(dtype)) && at(dC, 4 * es(dtype)) && N % 4 == 0;

@@ -4,6 +4,7 @@
 
 constexpr int SSM_CHUNK = 64;     // tokens of a chunk
 constexpr int SSM_MAX_N = 128;    // states per channel: the widest operand images in LDS
+static inline int ssm_padded_n(int N) { return N <= 32 ? 32 : N <= 64 ? 64 : 128; }
 
 struct SsmScanArgs {
   const void *x, *dt, *Bm, *Cm, *z;
@@ -12,11 +13,13 @@ struct SsmScanArgs {
   void* y;
   void* v;               // v before the gate, kept for the backward pass (or null)
   float* state_out;      // [B,H,P,N] or null
-  float* states;         // [nchunks][B,H,P,N]: the state before every chunk, kept for the backward pass (or null)
-  float* seg_state;      // [nseg][B,H,P,N]   (nseg > 1)
+  // Inner copies of states are padded to [B, H, pblocks * 64, NP] (NP: N up to 32, 64 or 128; what is added is zero), so that
+  // they are always read and written in whole aligned pieces.
+  float* states;         // [nchunks] of them: the state before every chunk, kept for the backward pass (or null)
+  float* seg_state;      // [nseg]    (nseg > 1)
   double* seg_decay;     // [nseg][B,H], base-2
   long sxb, sxt, sdb, sdt, sbb, sbt, scb, sct, szb, szt;
-  long seg_stride;       // B H P N
+  long seg_stride;       // floats of one padded copy
   int B, T, H, P, G, N, pblocks, nchunks, seg_chunks, nseg;
   bool vec_x, vec_bc, vec_z, vec_y, vec_state;   // wide accesses are aligned
 };
@@ -30,7 +33,7 @@ struct SsmBwdArgs {
   void *dB, *dC;               // [B,T,G,N]
   float *dA, *dD, *dbias;      // [H]
   float* dstate0;              // [B,H,P,N] or null
-  float* dstates;              // [nchunks][B,H,P,N]: gradient of the state behind every chunk
+  float* dstates;              // [nchunks], padded: gradient of the state behind every chunk
   float* dbc_part;             // [hsplit][2][B,T,G,N] (hsplit > 1)
   float* part;                 // [B * nchunks][H][3]: dA, dD, dbias of a chunk
   long syb, syt;
@@ -62,7 +65,7 @@ struct SsmConvArgs {
 int rvit_ssm_scan_fwd_impl(const SsmScanArgs& a, int dtype, hipStream_t st);
 int rvit_ssm_scan_bwd_impl(const SsmBwdArgs& a, int dtype, hipStream_t st);
 int rvit_ssm_scan_step_impl(const SsmStepArgs& a, int dtype, hipStream_t st);
-int rvit_ssm_join(float* seg_state, const double* seg_decay, const float* init, float* last, const SsmScanArgs& a, int reverse, hipStream_t st);
+int rvit_ssm_join(float* seg_state, const double* seg_decay, const float* init, const SsmScanArgs& a, int reverse, hipStream_t st);
 enum { SSM_CONV_FWD = 0, SSM_CONV_BWD = 1, SSM_CONV_STEP = 2 };
 int rvit_ssm_conv_impl(const SsmConvArgs& a, int dtype, int what, hipStream_t st);
 

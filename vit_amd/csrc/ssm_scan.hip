@@ -19,15 +19,55 @@ struct FwdLds {
   static constexpr int PN = NP + SsmOps<T>::PAD, PX = 64 + SsmOps<T>::PAD;
   static constexpr int GP = SsmOps<T>::template planes<2>();
   static constexpr int BS = 0, CS = BS + Q * PN, XS = CS + Q * PN, GS = XS + Q * PX, END = GS + GP * Q * PX;   // in elements of T
-  static constexpr int BYTES = END * (int)sizeof(T) + 5 * Q * (int)sizeof(float);
+  static constexpr int BYTES = END * (int)sizeof(T) + 10 * Q * (int)sizeof(float);
 };
+
+// scores of the 16 tokens of tile TILES - 1 against all up to them, decayed, times d_s, into Gs[t][s]; the tile beside the last
+// is written as zero where a step over 32 tokens will read it
+template <typename T, int NP, int TILES>
+__device__ __forceinline__ void scores(const T* Bs, const T* Cs, T* Gs, const float* sd, int tw, int q, int c) {
+  using L = FwdLds<T, NP>;
+  const float *shi = sd + Q, *slo = shi + Q;
+  const int t = 16 * tw + c;
+  f32x4 acc[TILES];
+#pragma unroll
+  for (int st = 0; st < TILES; ++st) acc[st] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int ks = 0; ks < NP; ks += 32) {
+    typename SsmOps<T>::Ex bf[TILES];
+#pragma unroll
+    for (int st = 0; st < TILES; ++st) bf[st] = ssm_row(Bs, L::PN, 16 * st + c, ks + 8 * q);
+    ssm_mma_rows(bf, ssm_row(Cs, L::PN, t, ks + 8 * q), acc);
+  }
+  const float thi = shi[t], tlo = slo[t];
+#pragma unroll
+  for (int st = 0; st < TILES; ++st) {
+    const int s = 16 * st + 4 * q;
+    const float4 hi = *reinterpret_cast<const float4*>(shi + s), lo = *reinterpret_cast<const float4*>(slo + s), d = *reinterpret_cast<const float4*>(sd + s);
+    float val[4];
+    val[0] = acc[st][0] * (ssm_exp2((thi - hi.x) + (tlo - lo.x)) * d.x);
+    val[1] = acc[st][1] * (ssm_exp2((thi - hi.y) + (tlo - lo.y)) * d.y);
+    val[2] = acc[st][2] * (ssm_exp2((thi - hi.z) + (tlo - lo.z)) * d.z);
+    val[3] = acc[st][3] * (ssm_exp2((thi - hi.w) + (tlo - lo.w)) * d.w);
+    if (st == TILES - 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) val[i] = s + i <= t ? val[i] : 0.f;      // a select: what is above the diagonal may be anything
+    }
+    ssm_put4<2>(Gs, Q * L::PX, t * L::PX + s, val);
+  }
+  if (TILES & 1) {
+    const float none[4] = {0.f, 0.f, 0.f, 0.f};
+    ssm_put4<2>(Gs, Q * L::PX, t * L::PX + 16 * TILES + 4 * q, none);
+  }
+}
 
 // One workgroup (four waves) per (sample, head, 64 channels, segment), chunk after chunk, the state in registers: wave w
 // holds S^T for channels 16w .. 16w+15, which is the A operand of exp(L_t) S C as it lies in the accumulators.
+// A chunk's images and decays are fetched and worked out while the chunk before it is computed.
 // YOUT = false: only the state a segment reaches from zero, and the segment's summed log decay (long sequences of few
-// rows are cut into segments, joined by ssm_join_kernel).
-template <typename T, int NP, bool YOUT>
-__global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(SsmScanArgs a) {
+// rows are cut into segments, joined by ssm_join_kernel).  VEC: all wide accesses are aligned and whole.
+template <typename T, int NP, bool YOUT, bool VEC>
+__global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_scan_fwd_kernel(SsmScanArgs a) {
   using O = SsmOps<T>;
   using L = FwdLds<T, NP>;
   constexpr int PN = L::PN, PX = L::PX, NT = NP / 16;
@@ -36,11 +76,7 @@ __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(SsmScanArgs a) {
   T* Cs = (T*)smem + L::CS;
   T* Xs = (T*)smem + L::XS;
   T* Gs = (T*)smem + L::GS;
-  float* sd = (float*)((T*)smem + L::END);   // d_t
-  float* shi = sd + Q;                       // L_t in base-2 units, high and low part
-  float* slo = shi + Q;
-  float* sw = slo + Q;                       // exp(L_Q - L_t) d_t
-  float* se = sw + Q;                        // exp(L_t)
+  float* decays = (float*)((T*)smem + L::END);   // two sets, by turns: d, L (high, low), exp(L_Q - L) d, exp(L)
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, q = lane >> 4, c = lane & 15;
   long id = blockIdx.x;
   const int seg = id % a.nseg; id /= a.nseg;
@@ -51,6 +87,8 @@ __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(SsmScanArgs a) {
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
   const int pw = min(64, a.P - pb * 64);           // channels of this block
   const int p0 = 16 * w;                           // this wave's first of them
+  const int tw = (blockIdx.x & 1) ? 3 - w : w;     // this wave's token tile in the score product: later ones have more to do, so
+                                                   // the two workgroups of a compute unit take them in opposite order
   const T* x = (const T*)a.x + b * a.sxb + (long)h * a.P + pb * 64;
   const T* Bm = (const T*)a.Bm + b * a.sbb + (long)g * a.N;
   const T* Cm = (const T*)a.Cm + b * a.scb + (long)g * a.N;
@@ -67,86 +105,103 @@ __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(SsmScanArgs a) {
   f32x4 S[NT];
   const bool has_p = p0 + c < pw;
   const long srow = (((long)b * a.H + h) * a.P + pb * 64 + p0 + c) * a.N;   // row of this lane's channel in [B,H,P,N]
-  {
-    const float* s0 = nullptr;
-    if (YOUT) {
-      if (a.nseg > 1) s0 = a.seg_state + seg * a.seg_stride + srow;          // written by the join
-      else if (a.state0) s0 = a.state0 + srow;
-    }
+  const long prow = ((((long)b * a.H + h) * a.pblocks + pb) * 64 + p0 + c) * NP;   // and in the padded copies
+  auto get_state = [&](const float* in, bool padded) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float v[4] = {0.f, 0.f, 0.f, 0.f};
-      if (s0 && has_p) ssm_ld4n(s0 + 16 * nt + 4 * q, a.N - 16 * nt - 4 * q, a.vec_state, v);
+      if (padded) ssm_ld4(in + prow + 16 * nt + 4 * q, v);
+      else if (has_p) ssm_ld4v<VEC>(in + srow + 16 * nt + 4 * q, a.N - 16 * nt - 4 * q, v);
       S[nt] = f32x4{v[0], v[1], v[2], v[3]};
     }
-  }
+  };
+  auto put_state = [&](float* out, bool padded) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float v[4] = {S[nt][0], S[nt][1], S[nt][2], S[nt][3]};
+      if (padded) ssm_st4(out + prow + 16 * nt + 4 * q, v);
+      else if (has_p) ssm_st4v<VEC>(out + srow + 16 * nt + 4 * q, a.N - 16 * nt - 4 * q, v);
+    }
+  };
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) S[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (YOUT && a.nseg > 1) get_state(a.seg_state + seg * a.seg_stride, true);     // written by the join
+  else if (YOUT && a.state0) get_state(a.state0, false);
   double total = 0.0;
+  // wave 0: the decays of a chunk from its dt (one token a lane)
+  auto fetch_dt = [&](int ch) { return dt[(long)min(ch * Q + lane, len - 1) * a.sdt]; };
+  auto decay = [&](T raw, int ch) {
+    float* sd = decays + (ch & 1) * 5 * Q;
+    const float d = ch * Q + lane < len ? ssm_softplus((float)raw + bias) : 0.f;
+    const double l2 = ssm_scan64((double)d * A2), end = ssm_last_lane(l2);
+    const float hi = (float)l2;
+    sd[lane] = d;
+    sd[Q + lane] = hi;
+    sd[2 * Q + lane] = (float)(l2 - (double)hi);
+    sd[3 * Q + lane] = ssm_exp2((float)(end - l2)) * d;
+    sd[4 * Q + lane] = ssm_exp2(hi);
+    total += end;
+  };
   const int c0 = seg * a.seg_chunks, c1 = min(a.nchunks, c0 + a.seg_chunks);
-  for (int ch = c0; ch < c1; ++ch) {
-    const int t0 = ch * Q;
-    const int live = min(max(len - t0, 0), Q);     // tokens of this chunk that exist
-    if (YOUT && a.states && has_p) {
-      float* out = a.states + (long)ch * a.seg_stride + srow;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float v[4] = {S[nt][0], S[nt][1], S[nt][2], S[nt][3]};
-        ssm_st4n(out + 16 * nt + 4 * q, a.N - 16 * nt - 4 * q, a.vec_state, v);
-      }
-    }
-    if (live == 0) {                               // behind the sequence: outputs are zero, the state stays
-      if (YOUT) {
-        for (int i = threadIdx.x; i < Q * 64; i += 256) {
-          const int t = t0 + (i >> 6), p = i & 63;
-          if (t < a.T && p < pw) { ssm_st(y + t * ldy + p, 0.f); if (v_out) ssm_st(v_out + t * ldy + p, 0.f); }
-        }
-      }
-      continue;
-    }
-    __syncthreads();
-    ssm_stage<T, 256, Q, NP>(Bs, PN, Bm + t0 * a.sbt, a.sbt, live, a.N, a.vec_bc);
-    if (YOUT) ssm_stage<T, 256, Q, NP>(Cs, PN, Cm + t0 * a.sct, a.sct, live, a.N, a.vec_bc);
-    ssm_stage<T, 256, Q, 64>(Xs, PX, x + t0 * a.sxt, a.sxt, live, pw, a.vec_x);
+  const int cl = min(c1, (len + Q - 1) / Q);       // chunks with tokens end here
+  SsmTile<T, 256, Q, NP, VEC> tb, tc;
+  SsmTile<T, 256, Q, 64, VEC> tx;
+  auto fetch = [&](int ch) {
+    const int live = min(len - ch * Q, Q);
+    tb.load(Bm + (long)ch * Q * a.sbt, a.sbt, live, a.N);
+    if (YOUT) tc.load(Cm + (long)ch * Q * a.sct, a.sct, live, a.N);
+    tx.load(x + (long)ch * Q * a.sxt, a.sxt, live, pw);
+  };
+  auto put = [&](int ch) {
+    const int live = min(len - ch * Q, Q);
+    tb.store(Bs, PN, live, a.N);
+    if (YOUT) tc.store(Cs, PN, live, a.N);
+    tx.store(Xs, PX, live, pw);
+  };
+  T raw = (T)0.f;
+  if (c0 < cl) {
+    fetch(c0);
     if (w == 0) {
-      const int t = t0 + lane;
-      const float d = lane < live ? ssm_softplus(ssm_ld(dt + t * a.sdt) + bias) : 0.f;
-      double l2 = (double)d * A2;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const double up = __shfl_up(l2, o, 64);
-        if (lane >= o) l2 += up;
-      }
-      const double end = __shfl(l2, 63, 64);
-      sd[lane] = d;
-      shi[lane] = (float)l2;
-      slo[lane] = (float)(l2 - (double)(float)l2);
-      sw[lane] = ssm_exp2((float)(end - l2)) * d;
-      se[lane] = ssm_exp2((float)l2);
-      total += end;
+      decay(fetch_dt(c0), c0);
+      raw = fetch_dt(c0 + 1);
     }
+    put(c0);
+  }
+  for (int ch = c0; ch < cl; ++ch) {
+    const int t0 = ch * Q;
+    const int live = min(len - t0, Q);             // tokens of this chunk that exist
+    const float* sd = decays + (ch & 1) * 5 * Q;
+    const float *shi = sd + Q, *slo = shi + Q, *sw = slo + Q, *se = sw + Q;
     __syncthreads();
-    const float eQ = se[Q - 1];
+    const bool more = ch + 1 < cl;
+    if (more) fetch(ch + 1);
+    if (YOUT && a.states) put_state(a.states + (long)ch * a.seg_stride, true);
+    if (w == 0 && more) {
+      decay(raw, ch + 1);
+      raw = fetch_dt(ch + 2);
+    }
+    SsmRaw4<T> zr[4];
     if (YOUT) {
-      // scores of the tokens 16w .. 16w+15 against all earlier ones, decayed, into Gs[t][s]
-      const int t = 16 * w + c;
-      const float thi = shi[t], tlo = slo[t];
-      for (int st = 0; st <= (w | 1); ++st) {
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        if (st <= w) {
+      // the gate of this wave's outputs, for the end of the chunk
+      const int p = p0 + 4 * q;
+      if (z) {
 #pragma unroll
-          for (int ks = 0; ks < NP; ks += 32)
-            acc = ssm_mma(ssm_row(Bs, PN, 16 * st + c, ks + 8 * q), ssm_row(Cs, PN, t, ks + 8 * q), acc);
+        for (int tt = 0; tt < 4; ++tt) {
+          const T* src = z + (long)(t0 + min(16 * tt + c, live - 1)) * a.szt;
+          if (VEC && a.vec_z) zr[tt].load(src + (p < pw ? p : 0));
+          else zr[tt].part(src + p, pw - p);
         }
-        float val[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int s = 16 * st + 4 * q + i;
-          val[i] = s <= t ? acc[i] * ssm_exp2((thi - shi[s]) + (tlo - slo[s])) * sd[s] : 0.f;
-        }
-        ssm_put4<2>(Gs, Q * PX, t * PX + 16 * st + 4 * q, val);
+      }
+      switch (tw) {
+        case 0: scores<T, NP, 1>(Bs, Cs, Gs, sd, tw, q, c); break;
+        case 1: scores<T, NP, 2>(Bs, Cs, Gs, sd, tw, q, c); break;
+        case 2: scores<T, NP, 3>(Bs, Cs, Gs, sd, tw, q, c); break;
+        default: scores<T, NP, 4>(Bs, Cs, Gs, sd, tw, q, c);
       }
       __syncthreads();
     }
-    if (p0 < pw) {
+    {
+      const float eQ = se[Q - 1];
       typename O::Ex xf[2];
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) xf[ks] = ssm_tr(Xs, PX, 32 * ks, p0, lane);
@@ -157,29 +212,40 @@ __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(SsmScanArgs a) {
 #pragma unroll
         for (int m = 0; m < NP / 32; ++m) {
           const float sv[8] = {S[2 * m][0], S[2 * m][1], S[2 * m][2], S[2 * m][3], S[2 * m + 1][0], S[2 * m + 1][1], S[2 * m + 1][2], S[2 * m + 1][3]};
-          const auto sf = O::template split<2>(sv);
+          typename O::Ex cf[4];
 #pragma unroll
-          for (int tt = 0; tt < 4; ++tt) acc[tt] = ssm_mma(sf, ssm_row_perm(Cs, PN, 16 * tt + c, 32 * m, q), acc[tt]);
+          for (int tt = 0; tt < 4; ++tt) cf[tt] = ssm_row_perm(Cs, PN, 16 * tt + c, 32 * m, q);
+          ssm_mma_cols(O::template split<2>(sv), cf, acc);
         }
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
-          acc[tt] *= se[16 * tt + c];
+        for (int tt = 0; tt < 4; ++tt) acc[tt] *= se[16 * tt + c];
 #pragma unroll
-          for (int ks = 0; ks <= tt / 2; ++ks)
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int tt = 2 * ks; tt < 4; ++tt)
             acc[tt] = ssm_mma(xf[ks], ssm_row_planes<2>(Gs, Q * PX, PX, 16 * tt + c, 32 * ks + 8 * q), acc[tt]);
-          const int tl = 16 * tt + c, t = t0 + tl, p = p0 + 4 * q;
-          if (t < a.T && p < pw) {
-            const bool is_live = tl < live;
-            float out[4], zv[4] = {0.f, 0.f, 0.f, 0.f};
+        const int p = p0 + 4 * q;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) out[i] = is_live ? acc[tt][i] + Dh * ssm_ld(Xs + tl * PX + p + i) : 0.f;
-            if (v_out) ssm_st4n(v_out + t * ldy + p, pw - p, a.vec_y, out);
-            if (z && is_live) {
-              ssm_ld4n(z + t * a.szt + p, pw - p, a.vec_z, zv);
+        for (int tt = 0; tt < 4; ++tt) {
+          const int tl = 16 * tt + c, t = t0 + tl;
+          float v[4], out[4], xv[4];
+          ssm_ld4(Xs + tl * PX + p, xv);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) out[i] *= zv[i] * ssm_sigmoid(zv[i]);
-            }
-            ssm_st4n(y + t * ldy + p, pw - p, a.vec_y, out);
+          for (int i = 0; i < 4; ++i) out[i] = v[i] = acc[tt][i] + Dh * xv[i];
+          if (z) {
+            float zv[4];
+            zr[tt].get(zv);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[i] *= zv[i] * ssm_sigmoid(zv[i]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {          // (a last chunk's rows behind the end)
+            v[i] = tl < live ? v[i] : 0.f;
+            out[i] = tl < live ? out[i] : 0.f;
+          }
+          if (t < a.T) {
+            if (v_out) ssm_st4v<VEC>(v_out + t * ldy + p, pw - p, v);
+            ssm_st4v<VEC>(y + t * ldy + p, pw - p, out);
           }
         }
       }
@@ -194,46 +260,49 @@ __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(SsmScanArgs a) {
         xw[ks] = O::template split<3>(v);
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        S[nt] *= eQ;
+      for (int nt = 0; nt < NT; ++nt) S[nt] *= eQ;
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) S[nt] = ssm_mma(ssm_tr(Bs, PN, 32 * ks, 16 * nt, lane), xw[ks], S[nt]);
+      for (int ks = 0; ks < 2; ++ks) {
+        typename O::Ex bf[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) bf[nt] = ssm_tr(Bs, PN, 32 * ks, 16 * nt, lane);
+        ssm_mma_rows(bf, xw[ks], S);
       }
     }
-  }
-  float* out = nullptr;
-  if (!YOUT) {
-    out = a.seg_state + seg * a.seg_stride + srow;
-    if (threadIdx.x == 0 && pb == 0) a.seg_decay[((long)seg * a.B + b) * a.H + h] = total;
-  } else if (a.state_out && seg == a.nseg - 1) {
-    out = a.state_out + srow;
-  }
-  if (out && has_p) {
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const float v[4] = {S[nt][0], S[nt][1], S[nt][2], S[nt][3]};
-      ssm_st4n(out + 16 * nt + 4 * q, a.N - 16 * nt - 4 * q, a.vec_state, v);
+    if (more) {
+      __syncthreads();
+      put(ch + 1);
     }
+  }
+  if (YOUT) {      // behind the sequence: outputs are zero
+    const int from = max(c0, cl) * Q, to = min(c1 * Q, a.T);
+    for (long i = threadIdx.x; i < (long)(to - from) * 64; i += 256) {
+      const int t = from + (int)(i >> 6), p = (int)(i & 63);
+      if (p < pw) { ssm_st(y + t * ldy + p, 0.f); if (v_out) ssm_st(v_out + t * ldy + p, 0.f); }
+    }
+    if (a.state_out && seg == a.nseg - 1) put_state(a.state_out, false);
+  } else {
+    put_state(a.seg_state + seg * a.seg_stride, true);
+    if (threadIdx.x == 0 && pb == 0) a.seg_decay[((long)seg * a.B + b) * a.H + h] = total;
   }
 }
 
 // Joins the segments: in place, the state a segment reached from zero becomes the state it starts from.  `reverse` runs from
-// the last segment to the first (the backward pass).  One thread per four state elements; the segments' values are loaded
-// ahead of the running product.
-__global__ __launch_bounds__(256) void ssm_join_kernel(float* seg_state, const double* seg_decay, const float* init, float* last,
-                                                       long n, int PN, long BH, int nseg, int reverse) {
+// the last segment to the first (the backward pass).  `init` [B,H,P,N] (or null) is what the first one starts from.
+__global__ __launch_bounds__(256) void ssm_join_kernel(float* seg_state, const double* seg_decay, const float* init, long n, int P, int N, int P64, int NP,
+                                                       long BH, int nseg, int reverse) {
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
-  const long bh = i / PN;
-  float run = init ? init[i] : 0.f;
-  for (int k = 0; k < nseg; ++k) {
-    const int s = reverse ? nseg - 1 - k : k;
+  const int k = i % NP, p = i / NP % P64;
+  const long bh = i / ((long)NP * P64);
+  float run = init && p < P && k < N ? init[(bh * P + p) * N + k] : 0.f;
+  for (int j = 0; j < nseg; ++j) {
+    const int s = reverse ? nseg - 1 - j : j;
     const float own = seg_state[s * n + i];
     const float f = ssm_exp2((float)seg_decay[s * BH + bh]);
     seg_state[s * n + i] = run;
     run = f * run + own;
   }
-  if (last) last[i] = run;
 }
 
 // One token per sample: the state is read once and written once, in place; HBM bound.  A workgroup takes one (sample, head);
@@ -279,33 +348,35 @@ __global__ __launch_bounds__(256) void ssm_scan_step_kernel(SsmStepArgs a) {
   }
 }
 
-template <typename T, int NP>
-int launch_fwd(const SsmScanArgs& a, bool yout, hipStream_t st) {
-  static RvitLdsLimit lim_y, lim_s;
+template <typename T, int NP, bool YOUT, bool VEC>
+int launch_fwd(const SsmScanArgs& a, hipStream_t st) {
+  static RvitLdsLimit lim;
   constexpr int bytes = FwdLds<T, NP>::BYTES;
-  const void* ky = (const void*)ssm_scan_fwd_kernel<T, NP, true>;
-  const void* ks = (const void*)ssm_scan_fwd_kernel<T, NP, false>;
-  if (int e = yout ? lim_y.ensure({ky}, bytes, "ssm_scan_fwd") : lim_s.ensure({ks}, bytes, "ssm_scan_fwd")) return e;
-  const dim3 grid((unsigned)((long)a.B * a.H * a.pblocks * a.nseg));
-  if (yout) hipLaunchKernelGGL((ssm_scan_fwd_kernel<T, NP, true>), grid, dim3(256), bytes, st, a);
-  else hipLaunchKernelGGL((ssm_scan_fwd_kernel<T, NP, false>), grid, dim3(256), bytes, st, a);
+  if (int e = lim.ensure({(const void*)ssm_scan_fwd_kernel<T, NP, YOUT, VEC>}, bytes, "ssm_scan_fwd")) return e;
+  hipLaunchKernelGGL((ssm_scan_fwd_kernel<T, NP, YOUT, VEC>), dim3((unsigned)((long)a.B * a.H * a.pblocks * a.nseg)), dim3(256), bytes, st, a);
   RVIT_CHECK_LAUNCH("ssm_scan_fwd");
   return RVIT_OK;
 }
 
+template <typename T, int NP>
+int launch_fwd_v(const SsmScanArgs& a, bool yout, hipStream_t st) {
+  const bool vec = a.vec_x && a.vec_bc && a.vec_state && (!yout || a.vec_y);
+  if (yout) return vec ? launch_fwd<T, NP, true, true>(a, st) : launch_fwd<T, NP, true, false>(a, st);
+  return vec ? launch_fwd<T, NP, false, true>(a, st) : launch_fwd<T, NP, false, false>(a, st);
+}
+
 template <typename T>
 int launch_fwd_n(const SsmScanArgs& a, bool yout, hipStream_t st) {
-  if (a.N <= 32) return launch_fwd<T, 32>(a, yout, st);
-  if (a.N <= 64) return launch_fwd<T, 64>(a, yout, st);
-  return launch_fwd<T, 128>(a, yout, st);
+  if (a.N <= 32) return launch_fwd_v<T, 32>(a, yout, st);
+  if (a.N <= 64) return launch_fwd_v<T, 64>(a, yout, st);
+  return launch_fwd_v<T, 128>(a, yout, st);
 }
 
 }  // namespace
 
-int rvit_ssm_join(float* seg_state, const double* seg_decay, const float* init, float* last, const SsmScanArgs& a, int reverse, hipStream_t st) {
-  const long n = (long)a.B * a.H * a.P * a.N;
-  hipLaunchKernelGGL(ssm_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, seg_state, seg_decay, init, last, n, a.P * a.N,
-                     (long)a.B * a.H, a.nseg, reverse);
+int rvit_ssm_join(float* seg_state, const double* seg_decay, const float* init, const SsmScanArgs& a, int reverse, hipStream_t st) {
+  hipLaunchKernelGGL(ssm_join_kernel, dim3((unsigned)((a.seg_stride + 255) / 256)), dim3(256), 0, st, seg_state, seg_decay, init, a.seg_stride, a.P, a.N,
+                     a.pblocks * 64, ssm_padded_n(a.N), (long)a.B * a.H, a.nseg, reverse);
   RVIT_CHECK_LAUNCH("ssm_join");
   return RVIT_OK;
 }
@@ -313,7 +384,7 @@ int rvit_ssm_join(float* seg_state, const double* seg_decay, const float* init, 
 int rvit_ssm_scan_fwd_impl(const SsmScanArgs& a, int dtype, hipStream_t st) {
   if (a.nseg > 1) {
     if (int e = dtype == RVIT_BF16 ? launch_fwd_n<bf16>(a, false, st) : launch_fwd_n<float>(a, false, st)) return e;
-    if (int e = rvit_ssm_join(a.seg_state, a.seg_decay, a.state0, nullptr, a, 0, st)) return e;
+    if (int e = rvit_ssm_join(a.seg_state, a.seg_decay, a.state0, a, 0, st)) return e;
   }
   return dtype == RVIT_BF16 ? launch_fwd_n<bf16>(a, true, st) : launch_fwd_n<float>(a, true, st);
 }

@@ -22,30 +22,15 @@ namespace {
 
 constexpr int Q = SSM_CHUNK;
 
-// d_t and the running log decay of a chunk, by one wave; returns the chunk's log decay (base 2, 64 bits)
-template <typename T>
-__device__ __forceinline__ double chunk_decay(const SsmScanArgs& f, const T* dt, long sdt, int live, double A2, float bias, int lane, float& raw,
-                                              float& d, double& l2) {
-  raw = lane < live ? ssm_ld(dt + lane * sdt) + bias : 0.f;
-  d = lane < live ? ssm_softplus(raw) : 0.f;
-  l2 = (double)d * A2;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double up = __shfl_up(l2, o, 64);
-    if (lane >= o) l2 += up;
-  }
-  return __shfl(l2, 63, 64);
-}
-
 // ---- sweep: dS before a chunk = exp(L_Q) dS behind it + sum_t exp(L_t) v'_t C_t^T ----
-template <typename T, int NP, bool OUT>
-__global__ __launch_bounds__(256) void ssm_scan_bwd_state_kernel(SsmBwdArgs a) {
+template <typename T, int NP, bool OUT, bool VEC>
+__global__ __launch_bounds__(256, 2) void ssm_scan_bwd_state_kernel(SsmBwdArgs a) {
   using O = SsmOps<T>;
   constexpr int PN = NP + O::PAD, PV = 68, NT = NP / 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* Cs = (T*)smem;
   float* Vs = (float*)(Cs + Q * PN);
-  float* se = Vs + Q * PV;
+  float* decays = Vs + Q * PV;                // two sets of exp(L_t), by turns
   const SsmScanArgs& f = a.f;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, q = lane >> 4, c = lane & 15;
   long id = blockIdx.x;
@@ -65,52 +50,90 @@ __global__ __launch_bounds__(256) void ssm_scan_bwd_state_kernel(SsmBwdArgs a) {
   f32x4 S[NT];
   const bool has_p = p0 + c < pw;
   const long srow = (((long)b * f.H + h) * f.P + pb * 64 + p0 + c) * f.N;
-  const float* s0 = OUT ? (f.nseg > 1 ? f.seg_state + seg * f.seg_stride : a.dstate_out) : nullptr;
+  const long prow = ((((long)b * f.H + h) * f.pblocks + pb) * 64 + p0 + c) * NP;
+  auto get_state = [&](const float* in, bool padded) {
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (s0 && has_p) ssm_ld4n(s0 + srow + 16 * nt + 4 * q, f.N - 16 * nt - 4 * q, f.vec_state, v);
-    S[nt] = f32x4{v[0], v[1], v[2], v[3]};
-  }
-  double total = 0.0;
-  const int c0 = seg * f.seg_chunks, c1 = min(f.nchunks, c0 + f.seg_chunks);
-  for (int ch = c1 - 1; ch >= c0; --ch) {
-    const int t0 = ch * Q;
-    const int live = min(max(len - t0, 0), Q);
-    if (live == 0) continue;
-    if (OUT && has_p) {
-      float* out = a.dstates + (long)ch * f.seg_stride + srow;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float v[4] = {S[nt][0], S[nt][1], S[nt][2], S[nt][3]};
-        ssm_st4n(out + 16 * nt + 4 * q, f.N - 16 * nt - 4 * q, f.vec_state, v);
-      }
-    }
-    __syncthreads();
-    ssm_stage<T, 256, Q, NP>(Cs, PN, Cm + t0 * f.sct, f.sct, live, f.N, f.vec_bc);
-    for (int i = threadIdx.x; i < Q * 16; i += 256) {
-      const int t = i >> 4, p = (i & 15) * 4;
+    for (int nt = 0; nt < NT; ++nt) {
       float v[4] = {0.f, 0.f, 0.f, 0.f};
-      if (t < live && p < pw) {
-        ssm_ld4n(dy + (t0 + t) * a.syt + p, pw - p, a.vec_dy, v);
-        if (z) {
-          float zv[4];
-          ssm_ld4n(z + (t0 + t) * f.szt + p, pw - p, f.vec_z, zv);
+      if (padded) ssm_ld4(in + prow + 16 * nt + 4 * q, v);
+      else if (has_p) ssm_ld4v<VEC>(in + srow + 16 * nt + 4 * q, f.N - 16 * nt - 4 * q, v);
+      S[nt] = f32x4{v[0], v[1], v[2], v[3]};
+    }
+  };
+  auto put_state = [&](float* out, bool padded) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] *= zv[j] * ssm_sigmoid(zv[j]);
-        }
+    for (int nt = 0; nt < NT; ++nt) {
+      const float v[4] = {S[nt][0], S[nt][1], S[nt][2], S[nt][3]};
+      if (padded) ssm_st4(out + prow + 16 * nt + 4 * q, v);
+      else if (has_p) ssm_st4v<VEC>(out + srow + 16 * nt + 4 * q, f.N - 16 * nt - 4 * q, v);
+    }
+  };
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) S[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (OUT && f.nseg > 1) get_state(f.seg_state + seg * f.seg_stride, true);
+  else if (OUT && a.dstate_out) get_state(a.dstate_out, false);
+  double total = 0.0;
+  auto fetch_dt = [&](int ch) { return dt[(long)min(max(ch, 0) * Q + lane, len - 1) * f.sdt]; };
+  auto decay = [&](T raw, int ch) {
+    const float d = ch * Q + lane < len ? ssm_softplus((float)raw + bias) : 0.f;
+    const double l2 = ssm_scan64((double)d * A2);
+    decays[(ch & 1) * Q + lane] = ssm_exp2((float)l2);
+    total += ssm_last_lane(l2);
+  };
+  const int c0 = seg * f.seg_chunks, cl = min(min(f.nchunks, c0 + f.seg_chunks), (len + Q - 1) / Q);
+  SsmTile<T, 256, Q, NP, VEC> tc;
+  SsmRaw4<T> dr[4], zr[4];                    // four pieces of four channels of dy and z
+  auto fetch = [&](int ch) {
+    const int live = min(len - ch * Q, Q);
+    tc.load(Cm + (long)ch * Q * f.sct, f.sct, live, f.N);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = i * 256 + threadIdx.x, p = (e & 15) * 4;
+      const long t = ch * Q + min(e >> 4, live - 1);
+      if (VEC) dr[i].load(dy + t * a.syt + (p < pw ? p : 0));
+      else dr[i].part(dy + t * a.syt + p, pw - p);
+      if (z && VEC && f.vec_z) zr[i].load(z + t * f.szt + (p < pw ? p : 0));
+      else if (z) zr[i].part(z + t * f.szt + p, pw - p);
+    }
+  };
+  auto put = [&](int ch) {
+    const int live = min(len - ch * Q, Q);
+    tc.store(Cs, PN, live, f.N);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = i * 256 + threadIdx.x, p = (e & 15) * 4, t = e >> 4;
+      float v[4], zv[4];
+      dr[i].get(v);
+      if (z) zr[i].get(zv);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (z) v[j] *= zv[j] * ssm_sigmoid(zv[j]);
+        if (t >= live || p >= pw) v[j] = 0.f;
       }
       *reinterpret_cast<float4*>(Vs + t * PV + p) = make_float4(v[0], v[1], v[2], v[3]);
     }
+  };
+  T raw = (T)0.f;
+  if (c0 < cl) {
+    fetch(cl - 1);
     if (w == 0) {
-      float raw, d;
-      double l2;
-      total += chunk_decay<T>(f, dt + t0 * f.sdt, f.sdt, live, A2, bias, lane, raw, d, l2);
-      se[lane] = ssm_exp2((float)l2);
+      decay(fetch_dt(cl - 1), cl - 1);
+      raw = fetch_dt(cl - 2);
     }
+    put(cl - 1);
+  }
+  for (int ch = cl - 1; ch >= c0; --ch) {
+    const float* se = decays + (ch & 1) * Q;
     __syncthreads();
-    const float eQ = se[Q - 1];
-    if (p0 < pw) {
+    const bool more = ch > c0;
+    if (more) fetch(ch - 1);
+    if (OUT) put_state(a.dstates + (long)ch * f.seg_stride, true);
+    if (w == 0 && more) {
+      decay(raw, ch - 1);
+      raw = fetch_dt(ch - 2);
+    }
+    {
+      const float eQ = se[Q - 1];
       typename O::template Cm<3> vw[2];
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
@@ -123,41 +146,42 @@ __global__ __launch_bounds__(256) void ssm_scan_bwd_state_kernel(SsmBwdArgs a) {
         vw[ks] = O::template split<3>(v);
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        S[nt] *= eQ;
+      for (int nt = 0; nt < NT; ++nt) S[nt] *= eQ;
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) S[nt] = ssm_mma(ssm_tr(Cs, PN, 32 * ks, 16 * nt, lane), vw[ks], S[nt]);
+      for (int ks = 0; ks < 2; ++ks) {
+        typename O::Ex cf[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) cf[nt] = ssm_tr(Cs, PN, 32 * ks, 16 * nt, lane);
+        ssm_mma_rows(cf, vw[ks], S);
       }
     }
+    if (more) {
+      __syncthreads();
+      put(ch - 1);
+    }
   }
-  float* out = nullptr;
   if (!OUT) {
-    out = f.seg_state + seg * f.seg_stride;
+    put_state(f.seg_state + seg * f.seg_stride, true);
     if (threadIdx.x == 0 && pb == 0) f.seg_decay[((long)seg * f.B + b) * f.H + h] = total;
   } else if (a.dstate0 && seg == 0) {
-    out = a.dstate0;
-  }
-  if (out && has_p) {
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const float v[4] = {S[nt][0], S[nt][1], S[nt][2], S[nt][3]};
-      ssm_st4n(out + srow + 16 * nt + 4 * q, f.N - 16 * nt - 4 * q, f.vec_state, v);
-    }
+    put_state(a.dstate0, false);
   }
 }
 
 // ---- the gradients of one chunk ----
-// One workgroup (eight waves) per (sample, chunk, group, part of the group's heads).  B and C stay in LDS over its heads and
-// the sums dB, dC over them in registers (wave: 16 states x 16 .. 64 tokens), so that shared heads cost no atomics.
+// One workgroup (eight waves) per (sample, chunk, group, part of the group's heads).  B, C and their scores G are there once
+// for all its heads, and the sums dB, dC over them stay in registers (wave: 16 states x 16 .. 64 tokens), so that shared
+// heads cost no atomics and no scratch where one workgroup takes them all.  A head's inputs are fetched while the head
+// before it is worked on, its states while its scores are.
 template <typename T, int NP>
 struct BwdLds {
   using O = SsmOps<T>;
   static constexpr int PN = NP + O::PAD, PX = 64 + O::PAD;
   static constexpr int VP = O::template planes<3>(), GP = O::template planes<2>();
   static constexpr int BS = 0, CS = BS + Q * PN, XS = CS + Q * PN, VS = XS + Q * PX, GS = VS + VP * Q * PX, WS = GS + GP * Q * PX, END = WS + GP * Q * PX;
-  // floats behind: d, hi, lo, exp(L_Q - L), exp(L): 5 Q;  column sums by token tile: 2 x 4 Q;  row sums by tile: 4 Q;
-  // rho by state tile: 8 Q;  sigma by channel tile: 4 Q;  <dS, S> and dD by wave: 16
-  static constexpr int FLOATS = 5 * Q + 8 * Q + 4 * Q + 8 * Q + 4 * Q + 16;
+  // floats behind: d, L (high, low), exp(L_Q - L), exp(L), sigmoid: 6 Q;  sums over a token tile: 2 x 4 Q;  row sums by tile:
+  // 4 Q;  rho by state tile: 8 Q;  sigma by channel tile: 4 Q;  <dS, S> by wave, dD by wave in two sets: 24
+  static constexpr int FLOATS = 6 * Q + 8 * Q + 4 * Q + 8 * Q + 4 * Q + 24;
   static constexpr int BYTES = END * (int)sizeof(T) + FLOATS * 4;
 };
 
@@ -173,12 +197,13 @@ __device__ __forceinline__ float groups_sum(float v) {   // over the four lanes 
   v += __shfl_xor(v, 16, 64);
   return v + __shfl_xor(v, 32, 64);
 }
+__device__ __forceinline__ float all_sum(float v) { return __shfl(ssm_scan64(v), 63, 64); }
 
-template <typename T, int NP>
-__global__ __launch_bounds__(512) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a) {
+template <typename T, int NP, bool VEC>
+__global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a) {
   using O = SsmOps<T>;
   using L = BwdLds<T, NP>;
-  constexpr int PN = L::PN, PX = L::PX, NT = NP / 16, CG = 8 / NT, CT = 4 / CG;   // column groups, column tiles of a wave
+  constexpr int PN = L::PN, PX = L::PX, PL = Q * PX, NT = NP / 16, CG = 8 / NT, CT = 4 / CG;   // column groups, column tiles of a wave
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* Bs = (T*)smem + L::BS;
   T* Cs = (T*)smem + L::CS;
@@ -191,12 +216,14 @@ __global__ __launch_bounds__(512) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a) {
   float* slo = shi + Q;
   float* sw = slo + Q;
   float* se = sw + Q;
-  float* r_e = se + Q;          // [4][Q] sum over a tile of tokens of (G W E)_ts
+  float* ssg = se + Q;
+  float* r_e = ssg + Q;         // [4][Q] sum over a tile of tokens of (G W E)_ts
   float* r_z = r_e + 4 * Q;     // [4][Q] sum over a tile's t >= u of its own s < u of M_ts
   float* r_m = r_z + 4 * Q;     // [4][Q] sum over a tile's s of M_ts, by s tile and t
   float* r_rho = r_m + 4 * Q;   // [8][Q]
   float* r_sig = r_rho + 8 * Q; // [4][Q]
-  float* r_w = r_sig + 4 * Q;   // [2][8]
+  float* r_k = r_sig + 4 * Q;   // [8]
+  float* r_d = r_k + 8;         // [2][8]
   const SsmScanArgs& f = a.f;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, q = lane >> 4, c = lane & 15;
   long id = blockIdx.x;
@@ -226,242 +253,357 @@ __global__ __launch_bounds__(512) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a) {
       if (threadIdx.x < 3) part[h * 3 + threadIdx.x] = 0.f;
     }
   } else {
-    ssm_stage<T, 512, Q, NP>(Bs, PN, (const T*)f.Bm + b * f.sbb + t0 * f.sbt + (long)g * f.N, f.sbt, live, f.N, f.vec_bc);
-    ssm_stage<T, 512, Q, NP>(Cs, PN, (const T*)f.Cm + b * f.scb + t0 * f.sct + (long)g * f.N, f.sct, live, f.N, f.vec_bc);
+    const T* gx = (const T*)f.x + b * f.sxb + t0 * f.sxt;
+    const T* gdy = (const T*)a.dy + b * a.syb + t0 * a.syt;
+    const T* gz = f.z ? (const T*)f.z + b * f.szb + t0 * f.szt : nullptr;
+    const T* gv = f.z ? (const T*)f.v + ((long)b * f.T + t0) * ldo : nullptr;
+    const T* gdt = (const T*)f.dt + b * f.sdb + (long)(t0 + min(lane, live - 1)) * f.sdt;
+    T* gdx = (T*)a.dx + ((long)b * f.T + t0) * ldo;
+    T* gdz = a.dz ? (T*)a.dz + ((long)b * f.T + t0) * ldo : nullptr;
+    // a head's x, dy, z, v: two pieces of four channels a thread, token row and row + 32
+    const int row = threadIdx.x >> 4, pq = (threadIdx.x & 15) * 4;
+    SsmRaw4<T> xr[2], dr[2], zr[2], vr[2];
+    T rawn = (T)0.f;
+    auto fetch = [&](int h, int pb) {
+      const int pw = min(64, f.P - pb * 64);
+      const long hp = (long)h * f.P + pb * 64;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int t = min(row + 32 * i, live - 1);
+        if (VEC) {
+          const int p = pq < pw ? pq : 0;
+          xr[i].load(gx + t * f.sxt + hp + p);
+          dr[i].load(gdy + t * a.syt + hp + p);
+          if (gz) {
+            if (f.vec_z) zr[i].load(gz + t * f.szt + hp + p);
+            else zr[i].part(gz + t * f.szt + hp + pq, pw - pq);
+            vr[i].load(gv + t * ldo + hp + p);
+          }
+        } else {
+          xr[i].part(gx + t * f.sxt + hp + pq, pw - pq);
+          dr[i].part(gdy + t * a.syt + hp + pq, pw - pq);
+          if (gz) {
+            zr[i].part(gz + t * f.szt + hp + pq, pw - pq);
+            vr[i].part(gv + t * ldo + hp + pq, pw - pq);
+          }
+        }
+      }
+      if (w == 0 && pb == 0) rawn = gdt[h];
+    };
+    fetch(h0, 0);
+    {
+      SsmTile<T, 512, Q, NP, VEC> tb, tc;
+      tb.load((const T*)f.Bm + b * f.sbb + t0 * f.sbt + (long)g * f.N, f.sbt, live, f.N);
+      tc.load((const T*)f.Cm + b * f.scb + t0 * f.sct + (long)g * f.N, f.sct, live, f.N);
+      tb.store(Bs, PN, live, f.N);
+      tc.store(Cs, PN, live, f.N);
+    }
     // tiles above the diagonal that a 32-wide step reads: (0, 1) and (2, 3); they stay zero
     for (int i = threadIdx.x; i < 2 * 16 * 16; i += 512) {
       const int k = i >> 8, o = ((i >> 4 & 15) + 32 * k) * PX + 16 + 32 * k + (i & 15);
 #pragma unroll
-      for (int pl = 0; pl < L::GP; ++pl) { Gs[pl * Q * PX + o] = (T)0.f; Ws[pl * Q * PX + o] = (T)0.f; }
+      for (int pl = 0; pl < L::GP; ++pl) { Gs[pl * PL + o] = (T)0.f; Ws[pl * PL + o] = (T)0.f; }
     }
+    __syncthreads();
+    // score tiles (tt, st), st <= tt: ten of them, wave w has number w and, of waves 0 and 1, number 8 + w
+    f32x4 Gt[2];
+#pragma unroll
+    for (int k2 = 0; k2 < 2; ++k2) {
+      Gt[k2] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const int k = w + 8 * k2;
+      if (k < 10) {
+        const int tt = k < 1 ? 0 : k < 3 ? 1 : k < 6 ? 2 : 3, st = k - tt * (tt + 1) / 2;
+#pragma unroll
+        for (int ks = 0; ks < NP; ks += 32)
+          Gt[k2] = ssm_mma(ssm_row(Bs, PN, 16 * st + c, ks + 8 * q), ssm_row(Cs, PN, 16 * tt + c, ks + 8 * q), Gt[k2]);
+      }
+    }
+    int turn = 0;
     for (int h = h0; h < h1; ++h) {
       const float Ah = f.A[h], Dh = f.D ? f.D[h] : 0.f;
-      float raw = 0.f, e_u = 0.f, da_u = 0.f, dD = 0.f;     // of token `lane`, in wave 0, over the channel blocks
-      for (int pb = 0; pb < f.pblocks; ++pb) {
+      float e_u = 0.f, da_u = 0.f, dD = 0.f;     // of token 63 - lane, in wave 0, over the channel blocks
+      for (int pb = 0; pb < f.pblocks; ++pb, turn ^= 1) {
         const int pw = min(64, f.P - pb * 64);
         const long hp = (long)h * f.P + pb * 64;
-        const long srow = (((long)ch * f.B + b) * f.H + h) * f.P * f.N + (long)pb * 64 * f.N;
+        // (the lane number anew for every head: its many LDS offsets are cheaper to work out again than to keep in registers)
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        const int q = lane >> 4, c = lane & 15;
+        // x and v' into LDS, dz out
+        float dd_part = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int t = row + 32 * i;
+          float xv[4], dv[4], dzv[4];
+          xr[i].get(xv);
+          dr[i].get(dv);
+          if (gz) {
+            float zv[4], vv[4];
+            zr[i].get(zv);
+            vr[i].get(vv);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float sg = ssm_sigmoid(zv[j]), zs = zv[j] * sg;
+              dzv[j] = dv[j] * vv[j] * (sg + zs * (1.f - sg));
+              dv[j] *= zs;
+            }
+          }
+          const bool in = t < live && pq < pw;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            xv[j] = in && (VEC || pq + j < pw) ? xv[j] : 0.f;
+            dv[j] = in && (VEC || pq + j < pw) ? dv[j] : 0.f;
+            dd_part += xv[j] * dv[j];
+          }
+          if (gdz && t < here) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) dzv[j] = in ? dzv[j] : 0.f;
+            ssm_st4v<VEC>(gdz + t * ldo + hp + pq, pw - pq, dzv);
+          }
+          ssm_put4<1>(Xs, 0, t * PX + pq, xv);
+          ssm_put4<3>(Vs, PL, t * PX + pq, dv);
+        }
+        dd_part = ssm_scan64(dd_part);
+        if (lane == 63) r_d[turn * 8 + w] = dd_part;
+        if (w == 0 && pb == 0) {
+          const float raw = (float)rawn + (f.dt_bias ? f.dt_bias[h] : 0.f);
+          const float d = lane < live ? ssm_softplus(raw) : 0.f;
+          const double l2 = ssm_scan64((double)d * ((double)Ah * 1.4426950408889634)), end = ssm_last_lane(l2);
+          const float hi = (float)l2;
+          sd[lane] = d;
+          shi[lane] = hi;
+          slo[lane] = (float)(l2 - (double)hi);
+          sw[lane] = ssm_exp2((float)(end - l2));
+          se[lane] = ssm_exp2(hi);
+          ssg[lane] = ssm_sigmoid(raw);
+        }
+        // the states of this head (padded copies): columns of this wave's 16 states (k = channels) for dB and dC, rows of its 16
+        // channels for dx
+        const long srow = (long)ch * f.seg_stride + (((long)b * f.H + h) * f.pblocks + pb) * 64 * NP;
         const float* S0 = f.states + srow;
         const float* dS = a.dstates + srow;
-        // state columns of this wave's 16 states, k = channels (A operands of the products with x and v')
-        float dsc[2][8], sc[2][8];
-        const int n = 16 * nt + c;
+        const int pt = w & 3, p0 = 16 * pt;
+        float dsc[2][8], sc[2][8], dsr[NP / 32][8];
+        {
+          const unsigned col = (8 * q * NP + 16 * nt + c) * 4, rowo = ((p0 + c) * NP + 8 * q) * 4;
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int p = 32 * ks + 8 * q + j;
-            const bool in = p < pw && n < f.N;
-            dsc[ks][j] = in ? dS[(long)p * f.N + n] : 0.f;
-            sc[ks][j] = in ? S0[(long)p * f.N + n] : 0.f;
+          for (int m = 0; m < NP / 32; ++m) {
+            ssm_ld4((const float*)((const char*)(dS + 32 * m) + rowo), reinterpret_cast<float(&)[4]>(dsr[m][0]));
+            ssm_ld4((const float*)((const char*)(dS + 32 * m + 4) + rowo), reinterpret_cast<float(&)[4]>(dsr[m][4]));
           }
-        __syncthreads();
-        float dd_part = 0.f;
-        for (int i = threadIdx.x; i < Q * 16; i += 512) {
-          const int t = i >> 4, p = (i & 15) * 4;
-          float xv[4] = {0.f, 0.f, 0.f, 0.f}, dv[4] = {0.f, 0.f, 0.f, 0.f};
-          if (p < pw && t < here) {
-            const long o = ((long)b * f.T + t0 + t) * ldo + hp + p;
-            float dzv[4] = {0.f, 0.f, 0.f, 0.f};
-            if (t < live) {
-              ssm_ld4n((const T*)f.x + b * f.sxb + (t0 + t) * f.sxt + hp + p, pw - p, f.vec_x, xv);
-              ssm_ld4n((const T*)a.dy + b * a.syb + (t0 + t) * a.syt + hp + p, pw - p, a.vec_dy, dv);
-              if (f.z) {
-                float zv[4], vv[4];
-                ssm_ld4n((const T*)f.z + b * f.szb + (t0 + t) * f.szt + hp + p, pw - p, f.vec_z, zv);
-                ssm_ld4n((const T*)f.v + o, pw - p, f.vec_y, vv);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const float sg = ssm_sigmoid(zv[j]);
-                  dzv[j] = dv[j] * vv[j] * (sg + zv[j] * sg * (1.f - sg));
-                  dv[j] *= zv[j] * sg;
-                }
-              }
+          for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) dd_part += xv[j] * dv[j];
-            }
-            if (a.dz) ssm_st4n((T*)a.dz + o, pw - p, a.vec_out, dzv);
-          }
-          ssm_put4<1>(Xs, 0, t * PX + p, xv);
-          ssm_put4<3>(Vs, Q * PX, t * PX + p, dv);
+            for (int j = 0; j < 8; ++j) dsc[ks][j] = *(const float*)((const char*)(dS + (32 * ks + j) * NP) + col);
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sc[ks][j] = *(const float*)((const char*)(S0 + (32 * ks + j) * NP) + col);
         }
-        dd_part = wave_sum(dd_part);
-        if (lane == 0) r_w[8 + w] = dd_part;
-        if (w == 0 && pb == 0) {
-          float d;
-          double l2;
-          const double end = chunk_decay<T>(f, (const T*)f.dt + b * f.sdb + t0 * f.sdt + h, f.sdt, live, (double)Ah * 1.4426950408889634,
-                                            f.dt_bias ? f.dt_bias[h] : 0.f, lane, raw, d, l2);
-          sd[lane] = d;
-          shi[lane] = (float)l2;
-          slo[lane] = (float)(l2 - (double)(float)l2);
-          sw[lane] = ssm_exp2((float)(end - l2));
-          se[lane] = ssm_exp2((float)l2);
-        }
+        __builtin_amdgcn_sched_barrier(0);
         __syncthreads();
-        // score tiles (tt, st), st <= tt: ten of them
-        for (int k = w; k < 10; k += 8) {
+        // score tiles
+#pragma unroll
+        for (int k2 = 0; k2 < 2; ++k2) {
+          const int k = w + 8 * k2;
+          if (k >= 10) break;
           const int tt = k < 1 ? 0 : k < 3 ? 1 : k < 6 ? 2 : 3, st = k - tt * (tt + 1) / 2;
-          f32x4 G = {0.f, 0.f, 0.f, 0.f}, W = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int ks = 0; ks < NP; ks += 32)
-            G = ssm_mma(ssm_row(Bs, PN, 16 * st + c, ks + 8 * q), ssm_row(Cs, PN, 16 * tt + c, ks + 8 * q), G);
+          const f32x4 G = Gt[k2];
+          f32x4 W = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int ks = 0; ks < 64; ks += 32)
-            W = ssm_mma(ssm_row(Xs, PX, 16 * st + c, ks + 8 * q), ssm_row_planes<3>(Vs, Q * PX, PX, 16 * tt + c, ks + 8 * q), W);
-          const int t = 16 * tt + c;
+            W = ssm_mma(ssm_row(Xs, PX, 16 * st + c, ks + 8 * q), ssm_row_planes<3>(Vs, PL, PX, 16 * tt + c, ks + 8 * q), W);
+          const int t = 16 * tt + c, s0 = 16 * st + 4 * q;
           const float thi = shi[t], tlo = slo[t];
-          float gv[4], wv[4], m[4], ec[4];
+          float hi[4], lo[4], d[4], gv[4], wv[4], m[4], ec[4];
+          ssm_ld4(shi + s0, hi);
+          ssm_ld4(slo + s0, lo);
+          ssm_ld4(sd + s0, d);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int s = 16 * st + 4 * q + i;
-            const float E = s <= t ? ssm_exp2((thi - shi[s]) + (tlo - slo[s])) : 0.f;
-            const float d = sd[s];
-            gv[i] = s <= t ? G[i] * E * d : 0.f;
-            wv[i] = s <= t ? W[i] * E * d : 0.f;
-            ec[i] = s <= t ? G[i] * W[i] * E : 0.f;
-            m[i] = ec[i] * d;
+            const bool on = s0 + i <= t;      // selects: what is above the diagonal may be anything
+            const float E = ssm_exp2((thi - hi[i]) + (tlo - lo[i]));
+            gv[i] = on ? G[i] * (E * d[i]) : 0.f;
+            wv[i] = on ? W[i] * (E * d[i]) : 0.f;
+            ec[i] = on ? G[i] * W[i] * E : 0.f;
+            m[i] = ec[i] * d[i];
           }
-          ssm_put4<2>(Gs, Q * PX, t * PX + 16 * st + 4 * q, gv);
-          ssm_put4<2>(Ws, Q * PX, t * PX + 16 * st + 4 * q, wv);
+          ssm_put4<2>(Gs, PL, t * PX + s0, gv);
+          ssm_put4<2>(Ws, PL, t * PX + s0, wv);
           // sums: of a row's tile, and of a row's part before u over the rows t >= u
           const float m4 = (m[0] + m[1]) + (m[2] + m[3]);
           const float u1 = __shfl_up(m4, 16, 64), u2 = __shfl_up(m4, 32, 64), u3 = __shfl_up(m4, 48, 64);
           float pre = (q >= 1 ? u1 : 0.f) + (q >= 2 ? u2 : 0.f) + (q >= 3 ? u3 : 0.f);
           if (q == 3) r_m[st * Q + t] = pre + m4;
+          float es[4], zs[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int s = 16 * st + 4 * q + i;
-            const float es = row16_sum(ec[i]), zs = row16_sum(s <= t ? pre : 0.f);
+            es[i] = row16_sum(ec[i]);
+            zs[i] = row16_sum(s0 + i <= t ? pre : 0.f);
             pre += m[i];
-            if (c == 0) { r_e[tt * Q + s] = es; r_z[tt * Q + s] = zs; }
+          }
+          if (c == 0) {
+            ssm_st4(r_e + tt * Q + s0, es);
+            ssm_st4(r_z + tt * Q + s0, zs);
           }
         }
         __syncthreads();
-        // dx: wave = 16 channels x 32 tokens
-        {
-          const int pt = w & 3, p0 = 16 * pt;
-          if (p0 < pw) {
-            f32x4 acc[2];
-            acc[0] = acc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (pb + 1 < f.pblocks) fetch(h, pb + 1);
+        else if (h + 1 < h1) fetch(h + 1, 0);
+        // dx: wave = 16 channels x 2 token tiles: 0 and 3, or 1 and 2
+        if (p0 < pw) {
+          const int st[2] = {w >> 2, 3 - (w >> 2)};
+          f32x4 acc[2];
+          acc[0] = acc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int m = 0; m < NP / 32; ++m) {
-              float v[8];
-              const int k = 32 * m + 8 * q;
-              float lo[4] = {0.f, 0.f, 0.f, 0.f}, hi[4] = {0.f, 0.f, 0.f, 0.f};
-              if (p0 + c < pw) {
-                ssm_ld4n(dS + (long)(p0 + c) * f.N + k, f.N - k, f.vec_state, lo);
-                ssm_ld4n(dS + (long)(p0 + c) * f.N + k + 4, f.N - k - 4, f.vec_state, hi);
-              }
+          for (int m = 0; m < NP / 32; ++m) {
+            typename O::Ex bf[2];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) { v[j] = lo[j]; v[4 + j] = hi[j]; }
-              const auto df = O::template split<3>(v);
-#pragma unroll
-              for (int k2 = 0; k2 < 2; ++k2) acc[k2] = ssm_mma(df, ssm_row(Bs, PN, 32 * (w >> 2) + 16 * k2 + c, k), acc[k2]);
-            }
-#pragma unroll
-            for (int k2 = 0; k2 < 2; ++k2) {
-              const int st = 2 * (w >> 2) + k2, s = 16 * st + c, p = p0 + 4 * q;
-              float sig = 0.f;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) sig += ssm_ld(Xs + s * PX + p + i) * acc[k2][i];
-              sig = groups_sum(sig);
-              if (q == 0) r_sig[pt * Q + s] = sig;
-              acc[k2] *= sw[s] * sd[s];
-              for (int ks = st / 2; ks < 2; ++ks)
-                acc[k2] = ssm_mma(ssm_tr_planes<2>(Vs, Q * PX, PX, 32 * ks, p0, lane), ssm_tr_planes<2>(Gs, Q * PX, PX, 32 * ks, 16 * st, lane), acc[k2]);
-              if (s < here && p < pw) {
-                float out[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  float v = 0.f;
-#pragma unroll
-                  for (int pl = L::VP - 1; pl >= 0; --pl) v += ssm_ld(Vs + pl * Q * PX + s * PX + p + i);
-                  out[i] = acc[k2][i] + Dh * v;
-                }
-                ssm_st4n((T*)a.dx + ((long)b * f.T + t0 + s) * ldo + hp + p, pw - p, a.vec_out, out);
-              }
-            }
-          } else if (lane < 32) {
-            r_sig[pt * Q + 32 * (w >> 2) + lane] = 0.f;
+            for (int k2 = 0; k2 < 2; ++k2) bf[k2] = ssm_row(Bs, PN, 16 * st[k2] + c, 32 * m + 8 * q);
+            ssm_mma_cols(O::template split<3>(dsr[m]), bf, acc);
           }
+          const int p = p0 + 4 * q;
+          float xv[2][4];
+#pragma unroll
+          for (int k2 = 0; k2 < 2; ++k2) {
+            const int s = 16 * st[k2] + c;
+            ssm_ld4(Xs + s * PX + p, xv[k2]);
+            const float sig = groups_sum((xv[k2][0] * acc[k2][0] + xv[k2][1] * acc[k2][1]) + (xv[k2][2] * acc[k2][2] + xv[k2][3] * acc[k2][3]));
+            if (q == 0) r_sig[pt * Q + s] = sig;
+            acc[k2] *= sw[s] * sd[s];
+          }
+          {
+            const auto vf = ssm_tr_planes<2>(Vs, PL, PX, 32, p0, lane);
+#pragma unroll
+            for (int k2 = 0; k2 < 2; ++k2) acc[k2] = ssm_mma(vf, ssm_tr_planes<2>(Gs, PL, PX, 32, 16 * st[k2], lane), acc[k2]);
+            acc[0] = ssm_mma(ssm_tr_planes<2>(Vs, PL, PX, 0, p0, lane), ssm_tr_planes<2>(Gs, PL, PX, 0, 16 * st[0], lane), acc[0]);
+          }
+#pragma unroll
+          for (int k2 = 0; k2 < 2; ++k2) {
+            const int s = 16 * st[k2] + c;
+            float out[4], pv[4], v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int pl = L::VP - 1; pl >= 0; --pl) {
+              ssm_ld4(Vs + pl * PL + s * PX + p, pv);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) v[i] += pv[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[i] = acc[k2][i] + Dh * v[i];
+            if (s < here) ssm_st4v<VEC>(gdx + s * ldo + hp + p, pw - p, out);
+          }
+        } else if (lane < 32) {
+          const int st = lane < 16 ? w >> 2 : 3 - (w >> 2);
+          r_sig[pt * Q + 16 * st + c] = 0.f;
         }
-        // dB, dC, rho, <dS, S>
+        __builtin_amdgcn_sched_barrier(0);
+        // dB, dC, rho, <dS, S>: wave = 16 states x CT token tiles
         {
-          const auto d0 = O::template split<2>(dsc[0]), d1 = O::template split<2>(dsc[1]);
-          const auto s0 = O::template split<3>(sc[0]), s1 = O::template split<3>(sc[1]);
           float kap = 0.f;
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (int j = 0; j < 8; ++j) kap += dsc[ks][j] * sc[ks][j];
-          kap = wave_sum(kap);
-          if (lane == 0) r_w[w] = cg == 0 ? kap : 0.f;
+          kap = ssm_scan64(kap);
+          if (lane == 63) r_k[w] = cg == 0 ? kap : 0.f;
+          {
+            f32x4 tb[CT];
 #pragma unroll
-          for (int k = 0; k < CT; ++k) {
-            const int ct = cg * CT + k, t = 16 * ct + c;
-            f32x4 tmp = {0.f, 0.f, 0.f, 0.f};
-            tmp = ssm_mma(d0, ssm_row(Xs, PX, t, 8 * q), tmp);
-            tmp = ssm_mma(d1, ssm_row(Xs, PX, t, 32 + 8 * q), tmp);
-            accB[k] += tmp * (sw[t] * sd[t]);
-            for (int ks = ct / 2; ks < 2; ++ks)
-              accB[k] = ssm_mma(ssm_tr(Cs, PN, 32 * ks, 16 * nt, lane), ssm_tr_planes<2>(Ws, Q * PX, PX, 32 * ks, 16 * ct, lane), accB[k]);
-            tmp = f32x4{0.f, 0.f, 0.f, 0.f};
-            tmp = ssm_mma(s0, ssm_row_planes<3>(Vs, Q * PX, PX, t, 8 * q), tmp);
-            tmp = ssm_mma(s1, ssm_row_planes<3>(Vs, Q * PX, PX, t, 32 + 8 * q), tmp);
-            tmp *= se[t];
-            float rho = 0.f;
+            for (int k = 0; k < CT; ++k) tb[k] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) rho += ssm_ld(Cs + t * PN + 16 * nt + 4 * q + i) * tmp[i];
-            rho = groups_sum(rho);
-            if (q == 0) r_rho[nt * Q + t] = rho;
-            accC[k] += tmp;
-            for (int ks = 0; ks <= ct / 2; ++ks)
-              accC[k] = ssm_mma(ssm_tr(Bs, PN, 32 * ks, 16 * nt, lane), ssm_row_planes<2>(Ws, Q * PX, PX, t, 32 * ks + 8 * q), accC[k]);
+            for (int ks = 0; ks < 2; ++ks) {
+              typename O::Ex xf[CT];
+#pragma unroll
+              for (int k = 0; k < CT; ++k) xf[k] = ssm_row(Xs, PX, 16 * (cg * CT + k) + c, 32 * ks + 8 * q);
+              ssm_mma_cols(O::template split<2>(dsc[ks]), xf, tb);
+            }
+#pragma unroll
+            for (int k = 0; k < CT; ++k) {
+              const int t = 16 * (cg * CT + k) + c;
+              accB[k] += tb[k] * (sw[t] * sd[t]);
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          {
+            constexpr int CP = CT < 2 ? 1 : 2;      // two token tiles at a time: their parts fill the registers
+            const auto s0 = O::template split<3>(sc[0]), s1 = O::template split<3>(sc[1]);
+#pragma unroll
+            for (int k = 0; k < CT; k += CP) {
+              f32x4 tc[CP];
+#pragma unroll
+              for (int m = 0; m < CP; ++m) tc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int ks = 0; ks < 2; ++ks) {
+                typename O::template Cm<3> vf[CP];
+#pragma unroll
+                for (int m = 0; m < CP; ++m) vf[m] = ssm_row_planes<3>(Vs, PL, PX, 16 * (cg * CT + k + m) + c, 32 * ks + 8 * q);
+                ssm_mma_cols(ks ? s1 : s0, vf, tc);
+              }
+#pragma unroll
+              for (int m = 0; m < CP; ++m) {
+                const int t = 16 * (cg * CT + k + m) + c;
+                tc[m] *= se[t];
+                float cv[4];
+                ssm_ld4(Cs + t * PN + 16 * nt + 4 * q, cv);
+                const float rho = groups_sum((cv[0] * tc[m][0] + cv[1] * tc[m][1]) + (cv[2] * tc[m][2] + cv[3] * tc[m][3]));
+                if (q == 0) r_rho[nt * Q + t] = rho;
+                accC[k + m] += tc[m];
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            const auto cf = ssm_tr(Cs, PN, 32 * ks, 16 * nt, lane);
+            const auto bf = ssm_tr(Bs, PN, 32 * ks, 16 * nt, lane);
+#pragma unroll
+            for (int k = 0; k < CT; ++k) {
+              const int ct = cg * CT + k;
+              if (ct / 2 <= ks) accB[k] = ssm_mma(cf, ssm_tr_planes<2>(Ws, PL, PX, 32 * ks, 16 * ct, lane), accB[k]);
+              if (ct / 2 >= ks) accC[k] = ssm_mma(bf, ssm_row_planes<2>(Ws, PL, PX, 16 * ct + c, 32 * ks + 8 * q), accC[k]);
+            }
           }
         }
         __syncthreads();
-        if (w == 0) {     // token `lane`
-          const int tl = lane >> 4;
-          float e = 0.f, zz = 0.f, sg = 0.f, rho = 0.f, kap = 0.f;
-          for (int tt = tl; tt < 4; ++tt) { e += r_e[tt * Q + lane]; zz += r_z[tt * Q + lane]; }
+        if (w == 0) {     // token u; the sums over t >= u run along the lanes
+          const int u = 63 - lane, tl = u >> 4;
+          float e = 0.f, zz = 0.f, sg = 0.f, sl = 0.f, rho = 0.f, kap = 0.f;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) sg += r_sig[k * Q + lane];
+          for (int tt = 0; tt < 4; ++tt) {
+            const float ev = r_e[tt * Q + u], zv = r_z[tt * Q + u];
+            e += tt >= tl ? ev : 0.f;
+            zz += tt >= tl ? zv : 0.f;
+          }
 #pragma unroll
-          for (int k = 0; k < NT; ++k) rho += r_rho[k * Q + lane];
+          for (int k = 0; k < 4; ++k) {
+            sg += r_sig[k * Q + u];
+            sl += r_sig[k * Q + lane];
+          }
 #pragma unroll
-          for (int k = 0; k < 8; ++k) { kap += r_w[k]; dD += r_w[8 + k]; }
-          sg *= sw[lane];
-          e += sg;
-          sg *= sd[lane];
-          // rows' sums over the s tiles before u's own, over t >= u
+          for (int k = 0; k < NT; ++k) rho += r_rho[k * Q + u];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) { kap += r_k[k]; dD += r_d[turn * 8 + k]; }
+          e += sg * sw[u];
+          // rows' sums over the s tiles before u's own
           float rs[3], run = 0.f;
 #pragma unroll
           for (int k = 0; k < 3; ++k) {
-            run += k <= tl ? r_m[k * Q + lane] : 0.f;
-            rs[k] = run;
+            const float mv = r_m[k * Q + u];
+            run += k <= tl ? mv : 0.f;
+            rs[k] = ssm_scan64(run);
           }
-          float suf[4] = {rho, rs[0], rs[1], rs[2]}, pre = sg;
-#pragma unroll
-          for (int o = 1; o < 64; o <<= 1) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float dn = __shfl_down(suf[k], o, 64);
-              if (lane + o < 64) suf[k] += dn;
-            }
-            const float up = __shfl_up(pre, o, 64);
-            if (lane >= o) pre += up;
-          }
-          const float before = __shfl_up(pre, 1, 64);
-          const float rows = tl == 0 ? 0.f : tl == 1 ? suf[1] : tl == 2 ? suf[2] : suf[3];
-          da_u += (zz + rows) + suf[0] + (lane > 0 ? before : 0.f) + se[Q - 1] * kap;
+          const float rows = tl == 0 ? 0.f : tl == 1 ? rs[0] : tl == 2 ? rs[1] : rs[2];
+          // sigma of the tokens before u
+          const float pre = ssm_scan64(sl * sw[lane] * sd[lane]);
+          const float before = __shfl(pre, max(u - 1, 0), 64);
+          da_u += (zz + rows) + ssm_scan64(rho) + (u > 0 ? before : 0.f) + se[Q - 1] * kap;
           e_u += e;
           if (pb == f.pblocks - 1) {
-            const bool ok = lane < live;
-            const float ddt = ok ? (e_u + Ah * da_u) * ssm_sigmoid(raw) : 0.f;
-            if (lane < here) ssm_st((T*)a.ddt + ((long)b * f.T + t0 + lane) * f.H + h, ddt);
-            const float sA = wave_sum(ok ? da_u * sd[lane] : 0.f), sb = wave_sum(ddt);
-            if (lane == 0) { part[h * 3] = sA; part[h * 3 + 1] = dD; part[h * 3 + 2] = sb; }
+            const bool ok = u < live;
+            const float ddt = ok ? (e_u + Ah * da_u) * ssg[u] : 0.f;
+            if (u < here) ssm_st((T*)a.ddt + ((long)b * f.T + t0 + u) * f.H + h, ddt);
+            const float sA = ssm_scan64(ok ? da_u * sd[u] : 0.f), sb = ssm_scan64(ddt);
+            if (lane == 63) { part[h * 3] = sA; part[h * 3 + 1] = dD; part[h * 3 + 2] = sb; }
           }
         }
       }
@@ -471,16 +613,16 @@ __global__ __launch_bounds__(512) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a) {
 #pragma unroll
   for (int k = 0; k < CT; ++k) {
     const int t = 16 * (cg * CT + k) + c, n = 16 * nt + 4 * q;
-    if (t < here && n < f.N) {
+    if (t < here) {
       const long o = (((long)b * f.T + t0 + t) * f.G + g) * f.N + n;
       const float vb[4] = {accB[k][0], accB[k][1], accB[k][2], accB[k][3]}, vc[4] = {accC[k][0], accC[k][1], accC[k][2], accC[k][3]};
       if (a.hsplit == 1) {
-        ssm_st4n((T*)a.dB + o, f.N - n, a.vec_dbc, vb);
-        ssm_st4n((T*)a.dC + o, f.N - n, a.vec_dbc, vc);
+        ssm_st4v<VEC>((T*)a.dB + o, f.N - n, vb);
+        ssm_st4v<VEC>((T*)a.dC + o, f.N - n, vc);
       } else {
         const long whole = (long)f.B * f.T * f.G * f.N;
-        ssm_st4n(a.dbc_part + 2 * hs * whole + o, f.N - n, a.vec_dbc, vb);
-        ssm_st4n(a.dbc_part + (2 * hs + 1) * whole + o, f.N - n, a.vec_dbc, vc);
+        ssm_st4v<VEC>(a.dbc_part + 2 * hs * whole + o, f.N - n, vb);
+        ssm_st4v<VEC>(a.dbc_part + (2 * hs + 1) * whole + o, f.N - n, vc);
       }
     }
   }
@@ -519,23 +661,23 @@ __global__ __launch_bounds__(256) void ssm_head_sum_kernel(const float* part, fl
   }
 }
 
-template <typename T, int NP>
+template <typename T, int NP, bool VEC>
 int launch_bwd(const SsmBwdArgs& a, hipStream_t st) {
   static RvitLdsLimit lim_o, lim_s, lim_c;
   const SsmScanArgs& f = a.f;
-  constexpr int sb = Q * (NP + SsmOps<T>::PAD) * (int)sizeof(T) + (Q * 68 + Q) * 4, cb = BwdLds<T, NP>::BYTES;
-  if (int e = lim_o.ensure({(const void*)ssm_scan_bwd_state_kernel<T, NP, true>}, sb, "ssm_scan_bwd_state")) return e;
-  if (int e = lim_s.ensure({(const void*)ssm_scan_bwd_state_kernel<T, NP, false>}, sb, "ssm_scan_bwd_state")) return e;
-  if (int e = lim_c.ensure({(const void*)ssm_scan_bwd_chunk_kernel<T, NP>}, cb, "ssm_scan_bwd_chunk")) return e;
+  constexpr int sb = Q * (NP + SsmOps<T>::PAD) * (int)sizeof(T) + (Q * 68 + 2 * Q) * 4, cb = BwdLds<T, NP>::BYTES;
+  if (int e = lim_o.ensure({(const void*)ssm_scan_bwd_state_kernel<T, NP, true, VEC>}, sb, "ssm_scan_bwd_state")) return e;
+  if (int e = lim_s.ensure({(const void*)ssm_scan_bwd_state_kernel<T, NP, false, VEC>}, sb, "ssm_scan_bwd_state")) return e;
+  if (int e = lim_c.ensure({(const void*)ssm_scan_bwd_chunk_kernel<T, NP, VEC>}, cb, "ssm_scan_bwd_chunk")) return e;
   const dim3 grid((unsigned)((long)f.B * f.H * f.pblocks * f.nseg));
   if (f.nseg > 1) {
-    hipLaunchKernelGGL((ssm_scan_bwd_state_kernel<T, NP, false>), grid, dim3(256), sb, st, a);
+    hipLaunchKernelGGL((ssm_scan_bwd_state_kernel<T, NP, false, VEC>), grid, dim3(256), sb, st, a);
     RVIT_CHECK_LAUNCH("ssm_scan_bwd_state");
-    if (int e = rvit_ssm_join(f.seg_state, f.seg_decay, a.dstate_out, nullptr, f, 1, st)) return e;
+    if (int e = rvit_ssm_join(f.seg_state, f.seg_decay, a.dstate_out, f, 1, st)) return e;
   }
-  hipLaunchKernelGGL((ssm_scan_bwd_state_kernel<T, NP, true>), grid, dim3(256), sb, st, a);
+  hipLaunchKernelGGL((ssm_scan_bwd_state_kernel<T, NP, true, VEC>), grid, dim3(256), sb, st, a);
   RVIT_CHECK_LAUNCH("ssm_scan_bwd_state");
-  hipLaunchKernelGGL((ssm_scan_bwd_chunk_kernel<T, NP>), dim3((unsigned)((long)f.B * f.nchunks * f.G * a.hsplit)), dim3(512), cb, st, a);
+  hipLaunchKernelGGL((ssm_scan_bwd_chunk_kernel<T, NP, VEC>), dim3((unsigned)((long)f.B * f.nchunks * f.G * a.hsplit)), dim3(512), cb, st, a);
   RVIT_CHECK_LAUNCH("ssm_scan_bwd_chunk");
   const long whole = (long)f.B * f.T * f.G * f.N;
   if (a.hsplit > 1) {
@@ -549,11 +691,18 @@ int launch_bwd(const SsmBwdArgs& a, hipStream_t st) {
   return RVIT_OK;
 }
 
+template <typename T, int NP>
+int launch_bwd_v(const SsmBwdArgs& a, hipStream_t st) {
+  const SsmScanArgs& f = a.f;
+  const bool vec = f.vec_x && f.vec_bc && f.vec_state && (!f.z || f.vec_y) && a.vec_dy && a.vec_out && a.vec_dbc;
+  return vec ? launch_bwd<T, NP, true>(a, st) : launch_bwd<T, NP, false>(a, st);
+}
+
 template <typename T>
 int launch_bwd_n(const SsmBwdArgs& a, hipStream_t st) {
-  if (a.f.N <= 32) return launch_bwd<T, 32>(a, st);
-  if (a.f.N <= 64) return launch_bwd<T, 64>(a, st);
-  return launch_bwd<T, 128>(a, st);
+  if (a.f.N <= 32) return launch_bwd_v<T, 32>(a, st);
+  if (a.f.N <= 64) return launch_bwd_v<T, 64>(a, st);
+  return launch_bwd_v<T, 128>(a, st);
 }
 
 }  // namespace
