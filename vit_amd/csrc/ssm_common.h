@@ -90,7 +90,7 @@ template <int M> __device__ __forceinline__ void ssm_mma_cols(const SsmF8& a, co
 // ---- operand types by input type ----
 template <typename T> struct SsmOps;
 template <> struct SsmOps<bf16> {
-  static constexpr int PAD = 8;                      // elements behind an LDS row: 16 bytes, rows start on other banks
+  static constexpr int PAD = 8;                      // elements behind an LDS row: rows start 16 bytes apart in the banks
   template <int NS> using Cm = SsmB8<NS>;
   using Ex = bf16x8;
   template <int NS> static constexpr int planes() { return NS; }

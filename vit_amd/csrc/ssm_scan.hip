@@ -16,9 +16,12 @@ constexpr int Q = SSM_CHUNK;
 
 template <typename T, int NP>
 struct FwdLds {
-  static constexpr int PN = NP + SsmOps<T>::PAD, PX = 64 + SsmOps<T>::PAD;
+  // Pitches: images with transposing reads (four rows of 32 bytes at a time) want rows 32 bytes apart in the banks, images that
+  // are only read along rows 16: with 32 everywhere the score and C reads collide half as often again.
+  static constexpr int SLIM = SsmOps<T>::PAD, WIDE = sizeof(T) == 2 ? 16 : 4;
+  static constexpr int PB = NP + WIDE, PC = NP + SLIM, PX = 64 + WIDE, PG = 64 + SLIM;
   static constexpr int GP = SsmOps<T>::template planes<2>();
-  static constexpr int BS = 0, CS = BS + Q * PN, XS = CS + Q * PN, GS = XS + Q * PX, END = GS + GP * Q * PX;   // in elements of T
+  static constexpr int BS = 0, CS = BS + Q * PB, XS = CS + Q * PC, GS = XS + Q * PX, END = GS + GP * Q * PG;   // in elements of T
   static constexpr int BYTES = END * (int)sizeof(T) + 10 * Q * (int)sizeof(float);
 };
 
@@ -36,8 +39,8 @@ __device__ __forceinline__ void scores(const T* Bs, const T* Cs, T* Gs, const fl
   for (int ks = 0; ks < NP; ks += 32) {
     typename SsmOps<T>::Ex bf[TILES];
 #pragma unroll
-    for (int st = 0; st < TILES; ++st) bf[st] = ssm_row(Bs, L::PN, 16 * st + c, ks + 8 * q);
-    ssm_mma_rows(bf, ssm_row(Cs, L::PN, t, ks + 8 * q), acc);
+    for (int st = 0; st < TILES; ++st) bf[st] = ssm_row(Bs, L::PB, 16 * st + c, ks + 8 * q);
+    ssm_mma_rows(bf, ssm_row(Cs, L::PC, t, ks + 8 * q), acc);
   }
   const float thi = shi[t], tlo = slo[t];
 #pragma unroll
@@ -53,11 +56,11 @@ __device__ __forceinline__ void scores(const T* Bs, const T* Cs, T* Gs, const fl
 #pragma unroll
       for (int i = 0; i < 4; ++i) val[i] = s + i <= t ? val[i] : 0.f;      // a select: what is above the diagonal may be anything
     }
-    ssm_put4<2>(Gs, Q * L::PX, t * L::PX + s, val);
+    ssm_put4<2>(Gs, Q * L::PG, t * L::PG + s, val);
   }
   if (TILES & 1) {
     const float none[4] = {0.f, 0.f, 0.f, 0.f};
-    ssm_put4<2>(Gs, Q * L::PX, t * L::PX + 16 * TILES + 4 * q, none);
+    ssm_put4<2>(Gs, Q * L::PG, t * L::PG + 16 * TILES + 4 * q, none);
   }
 }
 
@@ -70,7 +73,7 @@ template <typename T, int NP, bool YOUT, bool VEC>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_scan_fwd_kernel(SsmScanArgs a) {
   using O = SsmOps<T>;
   using L = FwdLds<T, NP>;
-  constexpr int PN = L::PN, PX = L::PX, NT = NP / 16;
+  constexpr int PB = L::PB, PC = L::PC, PX = L::PX, PG = L::PG, NT = NP / 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* Bs = (T*)smem + L::BS;
   T* Cs = (T*)smem + L::CS;
@@ -154,8 +157,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_
   };
   auto put = [&](int ch) {
     const int live = min(len - ch * Q, Q);
-    tb.store(Bs, PN, live, a.N);
-    if (YOUT) tc.store(Cs, PN, live, a.N);
+    tb.store(Bs, PB, live, a.N);
+    if (YOUT) tc.store(Cs, PC, live, a.N);
     tx.store(Xs, PX, live, pw);
   };
   T raw = (T)0.f;
@@ -214,7 +217,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_
           const float sv[8] = {S[2 * m][0], S[2 * m][1], S[2 * m][2], S[2 * m][3], S[2 * m + 1][0], S[2 * m + 1][1], S[2 * m + 1][2], S[2 * m + 1][3]};
           typename O::Ex cf[4];
 #pragma unroll
-          for (int tt = 0; tt < 4; ++tt) cf[tt] = ssm_row_perm(Cs, PN, 16 * tt + c, 32 * m, q);
+          for (int tt = 0; tt < 4; ++tt) cf[tt] = ssm_row_perm(Cs, PC, 16 * tt + c, 32 * m, q);
           ssm_mma_cols(O::template split<2>(sv), cf, acc);
         }
 #pragma unroll
@@ -223,7 +226,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
           for (int tt = 2 * ks; tt < 4; ++tt)
-            acc[tt] = ssm_mma(xf[ks], ssm_row_planes<2>(Gs, Q * PX, PX, 16 * tt + c, 32 * ks + 8 * q), acc[tt]);
+            acc[tt] = ssm_mma(xf[ks], ssm_row_planes<2>(Gs, Q * PG, PG, 16 * tt + c, 32 * ks + 8 * q), acc[tt]);
         const int p = p0 + 4 * q;
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
@@ -265,7 +268,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_
       for (int ks = 0; ks < 2; ++ks) {
         typename O::Ex bf[NT];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) bf[nt] = ssm_tr(Bs, PN, 32 * ks, 16 * nt, lane);
+        for (int nt = 0; nt < NT; ++nt) bf[nt] = ssm_tr(Bs, PB, 32 * ks, 16 * nt, lane);
         ssm_mma_rows(bf, xw[ks], S);
       }
     }

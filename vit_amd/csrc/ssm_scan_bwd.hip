@@ -179,10 +179,15 @@ struct BwdLds {
   static constexpr int PN = NP + O::PAD, PX = 64 + O::PAD;
   static constexpr int VP = O::template planes<3>(), GP = O::template planes<2>();
   static constexpr int BS = 0, CS = BS + Q * PN, XS = CS + Q * PN, VS = XS + Q * PX, GS = VS + VP * Q * PX, WS = GS + GP * Q * PX, END = WS + GP * Q * PX;
-  // floats behind: d, L (high, low), exp(L_Q - L), exp(L), sigmoid: 6 Q;  sums over a token tile: 2 x 4 Q;  row sums by tile:
-  // 4 Q;  rho by state tile: 8 Q;  sigma by channel tile: 4 Q;  <dS, S> by wave, dD by wave in two sets: 24
-  static constexpr int FLOATS = 6 * Q + 8 * Q + 4 * Q + 8 * Q + 4 * Q + 24;
-  static constexpr int BYTES = END * (int)sizeof(T) + FLOATS * 4;
+  // floats behind: two sets, by turns, of d, L (high, low), exp(L_Q - L), exp(L), sigmoid: 6 Q, of sums over a token tile: 2 x
+  // 4 Q, and of row sums by tile: 4 Q;  rho by state tile: 8 Q;  sigma by channel tile: 4 Q;  <dS, S> by wave, dD by wave (two
+  // sets): 24
+  static constexpr int SET = 18 * Q, FLOATS = 2 * SET + 8 * Q + 4 * Q + 24;
+  // dS as an fp32 image where it fits: fetched once, in whole lines, a head ahead; else (fp32, 128 states) straight from memory
+  // in both of its fragment layouts
+  static constexpr int PS = NP + 4, DS = END * (int)sizeof(T) + FLOATS * 4;
+  static constexpr bool DS_LDS = DS + Q * PS * 4 <= 160 * 1024;
+  static constexpr int BYTES = DS + (DS_LDS ? Q * PS * 4 : 0);
 };
 
 // sum over the 16 lanes of a row, in all of them (data-parallel moves inside the vector ALU, no LDS)
@@ -211,19 +216,11 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
   T* Vs = (T*)smem + L::VS;
   T* Gs = (T*)smem + L::GS;
   T* Ws = (T*)smem + L::WS;
-  float* sd = (float*)((T*)smem + L::END);
-  float* shi = sd + Q;
-  float* slo = shi + Q;
-  float* sw = slo + Q;
-  float* se = sw + Q;
-  float* ssg = se + Q;
-  float* r_e = ssg + Q;         // [4][Q] sum over a tile of tokens of (G W E)_ts
-  float* r_z = r_e + 4 * Q;     // [4][Q] sum over a tile's t >= u of its own s < u of M_ts
-  float* r_m = r_z + 4 * Q;     // [4][Q] sum over a tile's s of M_ts, by s tile and t
-  float* r_rho = r_m + 4 * Q;   // [8][Q]
-  float* r_sig = r_rho + 8 * Q; // [4][Q]
-  float* r_k = r_sig + 4 * Q;   // [8]
-  float* r_d = r_k + 8;         // [2][8]
+  float* sets = (float*)((T*)smem + L::END);
+  float* r_rho = sets + 2 * L::SET; // [8][Q]
+  float* r_sig = r_rho + 8 * Q;     // [4][Q]
+  float* r_k = r_sig + 4 * Q;       // [8]
+  float* r_d = r_k + 8;             // [2][8]
   const SsmScanArgs& f = a.f;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, q = lane >> 4, c = lane & 15;
   long id = blockIdx.x;
@@ -263,21 +260,35 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
     // a head's x, dy, z, v: two pieces of four channels a thread, token row and row + 32
     const int row = threadIdx.x >> 4, pq = (threadIdx.x & 15) * 4;
     SsmRaw4<T> xr[2], dr[2], zr[2], vr[2];
+    f32x4 dsn[NP / 32];
     T rawn = (T)0.f;
+    float* Ds = (float*)(smem + L::DS);
+    // (padded copies: [64 channels][NP] of a head are one piece)
+    auto padded = [&](int h, int pb) { return (long)ch * f.seg_stride + (((long)b * f.H + h) * f.pblocks + pb) * 64 * NP; };
     auto fetch = [&](int h, int pb) {
+      int tid = threadIdx.x;
+      asm volatile("" : "+v"(tid));
+      const int row = tid >> 4, pq = (tid & 15) * 4;
+      if constexpr (L::DS_LDS) {
+        const f32x4* src = (const f32x4*)(a.dstates + padded(h, pb));
+#pragma unroll
+        for (int i = 0; i < NP / 32; ++i) dsn[i] = (src + i * 512)[tid];
+      }
       const int pw = min(64, f.P - pb * 64);
       const long hp = (long)h * f.P + pb * 64;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int t = min(row + 32 * i, live - 1);
         if (VEC) {
-          const int p = pq < pw ? pq : 0;
-          xr[i].load(gx + t * f.sxt + hp + p);
-          dr[i].load(gdy + t * a.syt + hp + p);
+          // token strides are under 2^24 here: 32-bit offsets from a uniform address
+          const unsigned p = pq < pw ? pq : 0;
+          auto at = [&](const T* base, long st) { return (const T*)((const char*)(base + hp) + ((unsigned)t * (unsigned)st + p) * (unsigned)sizeof(T)); };
+          xr[i].load(at(gx, f.sxt));
+          dr[i].load(at(gdy, a.syt));
           if (gz) {
-            if (f.vec_z) zr[i].load(gz + t * f.szt + hp + p);
+            if (f.vec_z) zr[i].load(at(gz, f.szt));
             else zr[i].part(gz + t * f.szt + hp + pq, pw - pq);
-            vr[i].load(gv + t * ldo + hp + p);
+            vr[i].load(at(gv, ldo));
           }
         } else {
           xr[i].part(gx + t * f.sxt + hp + pq, pw - pq);
@@ -318,10 +329,57 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
           Gt[k2] = ssm_mma(ssm_row(Bs, PN, 16 * st + c, ks + 8 * q), ssm_row(Cs, PN, 16 * tt + c, ks + 8 * q), Gt[k2]);
       }
     }
-    int turn = 0;
+    int turn = 0, h_last = h0, pb_last = 0;
+    float e_u = 0.f, da_u = 0.f, dD = 0.f;       // of token 63 - lane, in wave 7, over the channel blocks of a head
+    // ddt of a head's tokens and its parts of dA, dD, dbias, by wave 7 while the others work on the next scores; the sums over
+    // t >= u run along the lanes
+    auto finish = [&](int h, int pb, int set) {
+      const float *sd = sets + set * L::SET, *sw = sd + 3 * Q, *se = sw + Q, *ssg = se + Q, *r_e = ssg + Q, *r_z = r_e + 4 * Q, *r_m = r_z + 4 * Q;
+      if (pb == 0) e_u = da_u = dD = 0.f;
+      int lane = threadIdx.x & 63;
+      asm volatile("" : "+v"(lane));
+      const int u = 63 - lane, tl = u >> 4;
+      float e = 0.f, zz = 0.f, sg = 0.f, sl = 0.f, rho = 0.f, kap = 0.f;
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+        const float ev = r_e[tt * Q + u], zv = r_z[tt * Q + u];
+        e += tt >= tl ? ev : 0.f;
+        zz += tt >= tl ? zv : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        sg += r_sig[k * Q + u];
+        sl += r_sig[k * Q + lane];
+      }
+#pragma unroll
+      for (int k = 0; k < NT; ++k) rho += r_rho[k * Q + u];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) { kap += r_k[k]; dD += r_d[set * 8 + k]; }
+      e += sg * sw[u];
+      // rows' sums over the s tiles before u's own
+      float rs[3], run = 0.f;
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        const float mv = r_m[k * Q + u];
+        run += k <= tl ? mv : 0.f;
+        rs[k] = ssm_scan64(run);
+      }
+      const float rows = tl == 0 ? 0.f : tl == 1 ? rs[0] : tl == 2 ? rs[1] : rs[2];
+      // sigma of the tokens before u
+      const float pre = ssm_scan64(sl * sw[lane] * sd[lane]);
+      const float before = __shfl(pre, max(u - 1, 0), 64);
+      da_u += (zz + rows) + ssm_scan64(rho) + (u > 0 ? before : 0.f) + se[Q - 1] * kap;
+      e_u += e;
+      if (pb == f.pblocks - 1) {
+        const bool ok = u < live;
+        const float ddt = ok ? (e_u + f.A[h] * da_u) * ssg[u] : 0.f;
+        if (u < here) ssm_st((T*)a.ddt + ((long)b * f.T + t0 + u) * f.H + h, ddt);
+        const float sA = ssm_scan64(ok ? da_u * sd[u] : 0.f), sb = ssm_scan64(ddt);
+        if (lane == 63) { part[h * 3] = sA; part[h * 3 + 1] = dD; part[h * 3 + 2] = sb; }
+      }
+    };
     for (int h = h0; h < h1; ++h) {
       const float Ah = f.A[h], Dh = f.D ? f.D[h] : 0.f;
-      float e_u = 0.f, da_u = 0.f, dD = 0.f;     // of token 63 - lane, in wave 0, over the channel blocks
       for (int pb = 0; pb < f.pblocks; ++pb, turn ^= 1) {
         const int pw = min(64, f.P - pb * 64);
         const long hp = (long)h * f.P + pb * 64;
@@ -329,6 +387,10 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
         int lane = threadIdx.x & 63;
         asm volatile("" : "+v"(lane));
         const int q = lane >> 4, c = lane & 15;
+        float *sd = sets + turn * L::SET, *shi = sd + Q, *slo = shi + Q, *sw = slo + Q, *se = sw + Q, *ssg = se + Q;
+        float* r_e = ssg + Q;         // [4][Q] sum over a tile of tokens of (G W E)_ts
+        float* r_z = r_e + 4 * Q;     // [4][Q] sum over a tile's t >= u of its own s < u of M_ts
+        float* r_m = r_z + 4 * Q;     // [4][Q] sum over a tile's s of M_ts, by s tile and t
         // x and v' into LDS, dz out
         float dd_part = 0.f;
 #pragma unroll
@@ -365,7 +427,7 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
         }
         dd_part = ssm_scan64(dd_part);
         if (lane == 63) r_d[turn * 8 + w] = dd_part;
-        if (w == 0 && pb == 0) {
+        if (w == 0) {
           const float raw = (float)rawn + (f.dt_bias ? f.dt_bias[h] : 0.f);
           const float d = lane < live ? ssm_softplus(raw) : 0.f;
           const double l2 = ssm_scan64((double)d * ((double)Ah * 1.4426950408889634)), end = ssm_last_lane(l2);
@@ -377,31 +439,29 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
           se[lane] = ssm_exp2(hi);
           ssg[lane] = ssm_sigmoid(raw);
         }
-        // the states of this head (padded copies): columns of this wave's 16 states (k = channels) for dB and dC, rows of its 16
-        // channels for dx
-        const long srow = (long)ch * f.seg_stride + (((long)b * f.H + h) * f.pblocks + pb) * 64 * NP;
-        const float* S0 = f.states + srow;
-        const float* dS = a.dstates + srow;
-        const int pt = w & 3, p0 = 16 * pt;
-        float dsc[2][8], sc[2][8], dsr[NP / 32][8];
-        {
-          const unsigned col = (8 * q * NP + 16 * nt + c) * 4, rowo = ((p0 + c) * NP + 8 * q) * 4;
+        if constexpr (L::DS_LDS) {
+          int tid = threadIdx.x;
+          asm volatile("" : "+v"(tid));
 #pragma unroll
-          for (int m = 0; m < NP / 32; ++m) {
-            ssm_ld4((const float*)((const char*)(dS + 32 * m) + rowo), reinterpret_cast<float(&)[4]>(dsr[m][0]));
-            ssm_ld4((const float*)((const char*)(dS + 32 * m + 4) + rowo), reinterpret_cast<float(&)[4]>(dsr[m][4]));
+          for (int i = 0; i < NP / 32; ++i) {
+            const int e = i * 512 + tid;
+            *reinterpret_cast<f32x4*>(Ds + e / (NP / 4) * L::PS + e % (NP / 4) * 4) = dsn[i];
           }
-#pragma unroll
-          for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) dsc[ks][j] = *(const float*)((const char*)(dS + (32 * ks + j) * NP) + col);
-#pragma unroll
-          for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sc[ks][j] = *(const float*)((const char*)(S0 + (32 * ks + j) * NP) + col);
         }
+        const int pt = w & 3, p0 = 16 * pt;
         __builtin_amdgcn_sched_barrier(0);
         __syncthreads();
+        // this wave's 16 states of S as columns (k = channels), for dC
+        const unsigned col = 8 * q * NP + 16 * nt + c;
+        const float* dS = a.dstates + padded(h, pb);
+        float sc[2][8];
+        {
+          const float* S0 = f.states + padded(h, pb);
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sc[ks][j] = (S0 + (32 * ks + j) * NP)[col];
+        }
         // score tiles
 #pragma unroll
         for (int k2 = 0; k2 < 2; ++k2) {
@@ -447,9 +507,13 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
             ssm_st4(r_z + tt * Q + s0, zs);
           }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        if (w == 7 && (h > h0 || pb > 0)) finish(h_last, pb_last, turn ^ 1);
         __syncthreads();
-        if (pb + 1 < f.pblocks) fetch(h, pb + 1);
-        else if (h + 1 < h1) fetch(h + 1, 0);
+        {
+          const bool same = pb + 1 < f.pblocks;
+          if (same || h + 1 < h1) fetch(same ? h : h + 1, same ? pb + 1 : 0);
+        }
         // dx: wave = 16 channels x 2 token tiles: 0 and 3, or 1 and 2
         if (p0 < pw) {
           const int st[2] = {w >> 2, 3 - (w >> 2)};
@@ -460,7 +524,11 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
             typename O::Ex bf[2];
 #pragma unroll
             for (int k2 = 0; k2 < 2; ++k2) bf[k2] = ssm_row(Bs, PN, 16 * st[k2] + c, 32 * m + 8 * q);
-            ssm_mma_cols(O::template split<3>(dsr[m]), bf, acc);
+            float v[8];      // dS, rows of this wave's channels
+            const float* src = L::DS_LDS ? Ds + (p0 + c) * L::PS + 32 * m + 8 * q : dS + (p0 + c) * NP + 32 * m + 8 * q;
+            ssm_ld4(src, reinterpret_cast<float(&)[4]>(v[0]));
+            ssm_ld4(src + 4, reinterpret_cast<float(&)[4]>(v[4]));
+            ssm_mma_cols(O::template split<3>(v), bf, acc);
           }
           const int p = p0 + 4 * q;
           float xv[2][4];
@@ -499,7 +567,12 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
         __builtin_amdgcn_sched_barrier(0);
         // dB, dC, rho, <dS, S>: wave = 16 states x CT token tiles
         {
-          float kap = 0.f;
+          float kap = 0.f, dsc[2][8];      // dS, columns of this wave's states
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              dsc[ks][j] = L::DS_LDS ? Ds[(32 * ks + 8 * q + j) * L::PS + 16 * nt + c] : (dS + (32 * ks + j) * NP)[col];
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -565,49 +638,11 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
           }
         }
         __syncthreads();
-        if (w == 0) {     // token u; the sums over t >= u run along the lanes
-          const int u = 63 - lane, tl = u >> 4;
-          float e = 0.f, zz = 0.f, sg = 0.f, sl = 0.f, rho = 0.f, kap = 0.f;
-#pragma unroll
-          for (int tt = 0; tt < 4; ++tt) {
-            const float ev = r_e[tt * Q + u], zv = r_z[tt * Q + u];
-            e += tt >= tl ? ev : 0.f;
-            zz += tt >= tl ? zv : 0.f;
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            sg += r_sig[k * Q + u];
-            sl += r_sig[k * Q + lane];
-          }
-#pragma unroll
-          for (int k = 0; k < NT; ++k) rho += r_rho[k * Q + u];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) { kap += r_k[k]; dD += r_d[turn * 8 + k]; }
-          e += sg * sw[u];
-          // rows' sums over the s tiles before u's own
-          float rs[3], run = 0.f;
-#pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            const float mv = r_m[k * Q + u];
-            run += k <= tl ? mv : 0.f;
-            rs[k] = ssm_scan64(run);
-          }
-          const float rows = tl == 0 ? 0.f : tl == 1 ? rs[0] : tl == 2 ? rs[1] : rs[2];
-          // sigma of the tokens before u
-          const float pre = ssm_scan64(sl * sw[lane] * sd[lane]);
-          const float before = __shfl(pre, max(u - 1, 0), 64);
-          da_u += (zz + rows) + ssm_scan64(rho) + (u > 0 ? before : 0.f) + se[Q - 1] * kap;
-          e_u += e;
-          if (pb == f.pblocks - 1) {
-            const bool ok = u < live;
-            const float ddt = ok ? (e_u + Ah * da_u) * ssg[u] : 0.f;
-            if (u < here) ssm_st((T*)a.ddt + ((long)b * f.T + t0 + u) * f.H + h, ddt);
-            const float sA = ssm_scan64(ok ? da_u * sd[u] : 0.f), sb = ssm_scan64(ddt);
-            if (lane == 63) { part[h * 3] = sA; part[h * 3 + 1] = dD; part[h * 3 + 2] = sb; }
-          }
-        }
+        h_last = h;
+        pb_last = pb;
       }
     }
+    if (w == 7) finish(h_last, pb_last, turn ^ 1);
   }
   // accB, accC: states 16nt + 4q + i of token 16 ct + c
 #pragma unroll
