@@ -132,7 +132,8 @@ int rvit_ssm_scan_bwd(const void* x, int64_t sxb, int64_t sxt, const void* dt, i
   a.vec_dbc = at(dB, 4 * es(dtype)) && at(dC, 4 * es(dtype)) && N % 4 == 0;
   char* ws = (char*)workspace;
   take_segments(a.f, ws);
-  a.dstates = (float*)ws;
+  // (of one chunk without a gradient of its end there is nothing to sweep: dS is zero)
+  a.dstates = a.f.nchunks == 1 && !dstate_out && !dstate0 ? nullptr : (float*)ws;
   ws += round16((int64_t)a.f.nchunks * a.f.seg_stride * 4);
   a.part = (float*)ws;
   ws += round16((int64_t)B * a.f.nchunks * H * 12);

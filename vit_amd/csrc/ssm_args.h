@@ -33,7 +33,7 @@ struct SsmBwdArgs {
   void *dB, *dC;               // [B,T,G,N]
   float *dA, *dD, *dbias;      // [H]
   float* dstate0;              // [B,H,P,N] or null
-  float* dstates;              // [nchunks], padded: gradient of the state behind every chunk
+  float* dstates;              // [nchunks], padded: gradient of the state behind every chunk (null: zero)
   float* dbc_part;             // [hsplit][2][B,T,G,N] (hsplit > 1)
   float* part;                 // [B * nchunks][H][3]: dA, dD, dbias of a chunk
   long syb, syt;

@@ -272,7 +272,7 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
       if constexpr (L::DS_LDS) {
         const f32x4* src = (const f32x4*)(a.dstates + padded(h, pb));
 #pragma unroll
-        for (int i = 0; i < NP / 32; ++i) dsn[i] = (src + i * 512)[tid];
+        for (int i = 0; i < NP / 32; ++i) dsn[i] = a.dstates ? (src + i * 512)[tid] : f32x4{0.f, 0.f, 0.f, 0.f};
       }
       const int pw = min(64, f.P - pb * 64);
       const long hp = (long)h * f.P + pb * 64;
@@ -525,9 +525,14 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
 #pragma unroll
             for (int k2 = 0; k2 < 2; ++k2) bf[k2] = ssm_row(Bs, PN, 16 * st[k2] + c, 32 * m + 8 * q);
             float v[8];      // dS, rows of this wave's channels
-            const float* src = L::DS_LDS ? Ds + (p0 + c) * L::PS + 32 * m + 8 * q : dS + (p0 + c) * NP + 32 * m + 8 * q;
-            ssm_ld4(src, reinterpret_cast<float(&)[4]>(v[0]));
-            ssm_ld4(src + 4, reinterpret_cast<float(&)[4]>(v[4]));
+            if (L::DS_LDS || a.dstates) {
+              const float* src = L::DS_LDS ? Ds + (p0 + c) * L::PS + 32 * m + 8 * q : dS + (p0 + c) * NP + 32 * m + 8 * q;
+              ssm_ld4(src, reinterpret_cast<float(&)[4]>(v[0]));
+              ssm_ld4(src + 4, reinterpret_cast<float(&)[4]>(v[4]));
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] = 0.f;
+            }
             ssm_mma_cols(O::template split<3>(v), bf, acc);
           }
           const int p = p0 + 4 * q;
@@ -572,7 +577,7 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
           for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              dsc[ks][j] = L::DS_LDS ? Ds[(32 * ks + 8 * q + j) * L::PS + 16 * nt + c] : (dS + (32 * ks + j) * NP)[col];
+              dsc[ks][j] = L::DS_LDS ? Ds[(32 * ks + 8 * q + j) * L::PS + 16 * nt + c] : a.dstates ? (dS + (32 * ks + j) * NP)[col] : 0.f;
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -710,8 +715,10 @@ int launch_bwd(const SsmBwdArgs& a, hipStream_t st) {
     RVIT_CHECK_LAUNCH("ssm_scan_bwd_state");
     if (int e = rvit_ssm_join(f.seg_state, f.seg_decay, a.dstate_out, f, 1, st)) return e;
   }
-  hipLaunchKernelGGL((ssm_scan_bwd_state_kernel<T, NP, true, VEC>), grid, dim3(256), sb, st, a);
-  RVIT_CHECK_LAUNCH("ssm_scan_bwd_state");
+  if (a.dstates) {
+    hipLaunchKernelGGL((ssm_scan_bwd_state_kernel<T, NP, true, VEC>), grid, dim3(256), sb, st, a);
+    RVIT_CHECK_LAUNCH("ssm_scan_bwd_state");
+  }
   hipLaunchKernelGGL((ssm_scan_bwd_chunk_kernel<T, NP, VEC>), dim3((unsigned)((long)f.B * f.nchunks * f.G * a.hsplit)), dim3(512), cb, st, a);
   RVIT_CHECK_LAUNCH("ssm_scan_bwd_chunk");
   const long whole = (long)f.B * f.T * f.G * f.N;

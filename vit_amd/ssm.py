@@ -20,7 +20,8 @@ _same = contextlib.nullcontext()
 
 def _on(t: torch.Tensor):
     """The launch goes to the current device's stream: make t's device current where it is not."""
-    return _same if not t.is_cuda or t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    dev = t.get_device()
+    return _same if dev < 0 or dev == ops._raw_device() else torch.cuda.device(dev)
 
 
 def _packed(t: Optional[torch.Tensor], inner: int) -> Optional[torch.Tensor]:
@@ -28,7 +29,7 @@ def _packed(t: Optional[torch.Tensor], inner: int) -> Optional[torch.Tensor]:
     if t is None:
         return None
     step = 1
-    for d in range(1, inner + 1):
+    for d in range(1, min(inner, t.dim()) + 1):
         if t.shape[-d] != 1 and t.stride(-d) != step:
             return t.contiguous()
         step *= t.shape[-d]
@@ -36,7 +37,11 @@ def _packed(t: Optional[torch.Tensor], inner: int) -> Optional[torch.Tensor]:
 
 
 def _wants_grad(*ts: Optional[torch.Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _c(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -83,8 +88,7 @@ class _Conv(torch.autograd.Function):
                 if ds is not None:
                     ds.zero_() if dafter is None else ds.copy_(dafter)
             else:
-                ops.ssm_conv_bwd(x, weight, bias, dy, dx, dw, db, silu=ctx.silu, state=state, lengths=lengths, dstate_out=_c(dafter),
-                                 dstate=ds)
+                ops._ssm_conv_bwd(x, weight, bias, dy, dx, dw, db, ctx.silu, state, lengths, _c(dafter), ds)
         return dx, dw, db, None, ds, None, None
 
 
@@ -110,33 +114,38 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     return (y, after) if return_state else y
 
 
-@torch.no_grad()
 def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], state: torch.Tensor, *,
                      activation: Optional[str] = None) -> torch.Tensor:
     """causal_conv for one token: x [B,C], state [B,K-1,C] (advances in place); returns [B,C].  No gradient."""
+    silu = _silu(activation)
+    sig = ops._sig("ssm_conv_step", x, weight, bias, state)
+    if sig not in ops._SEEN:
+        x, sig = _packed(x, 1), None
     with _on(x):
-        x = _packed(x, 1)
-        return ops.ssm_conv_step(x, weight, bias, state, torch.empty(x.shape, dtype=x.dtype, device=x.device), silu=_silu(activation))
+        return ops.ssm_conv_step(x, weight, bias, state, silu=silu, sig=sig)
 
 
 # ---- selective scan -----------------------------------------------------------------------------------------------------
-def _scan_fwd(x, dt, A, Bm, Cm, D, z, dt_bias, state, lengths, want_state, train):
-    ops._scan_shapes("selective_scan", x, dt, A, Bm, Cm, D, z, dt_bias, False)
-    B, T, H, P = x.shape
-    G, N = Bm.shape[-2:]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    after = torch.empty(B, H, P, N, dtype=F32, device=x.device) if want_state else None
-    v = torch.empty_like(y) if train and z is not None else None
-    states = torch.empty(ops.ssm_scan_plan(B, T, H, P, G, N)[1], dtype=F32, device=x.device) if train else None
-    ops.ssm_scan(x, dt, A, Bm, Cm, D, z, dt_bias, y, state=state, state_out=after, lengths=lengths, v=v, states=states)
+def _scan_fwd(x, dt, A, Bm, Cm, D, z, dt_bias, state, lengths, want_state, train, sig=None):
+    after = v = states = None
+    if want_state or train:
+        ops._scan_shapes("selective_scan", x, dt, A, Bm, Cm, D, z, dt_bias, False) if sig is None else None
+        B, T, H, P = x.shape
+        G, N = Bm.shape[-2:]
+        if want_state:
+            after = torch.empty((B, H, P, N), dtype=F32, device=x.device)
+        if train:
+            v = None if z is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            states = torch.empty(ops.ssm_scan_plan(B, T, H, P, G, N)[1], dtype=F32, device=x.device)
+    y = ops.ssm_scan(x, dt, A, Bm, Cm, D, z, dt_bias, state=state, state_out=after, lengths=lengths, v=v, states=states, sig=sig)
     return y, after, v, states
 
 
 class _Scan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, dt, A, Bm, Cm, D, z, dt_bias, state, lengths, want_state):
+    def forward(ctx, x, dt, A, Bm, Cm, D, z, dt_bias, state, lengths, want_state, sig):
         with _on(x):
-            y, after, v, states = _scan_fwd(x, dt, A, Bm, Cm, D, z, dt_bias, state, lengths, want_state, True)
+            y, after, v, states = _scan_fwd(x, dt, A, Bm, Cm, D, z, dt_bias, state, lengths, want_state, True, sig)
         ctx.save_for_backward(x, dt, A, Bm, Cm, D, z, dt_bias, lengths, v, states)
         ctx.had_state = state is not None
         ctx.set_materialize_grads(False)
@@ -147,10 +156,13 @@ class _Scan(torch.autograd.Function):
     def backward(ctx, dy, dafter):
         x, dt, A, Bm, Cm, D, z, dt_bias, lengths, v, states = ctx.saved_tensors
         with _on(x):
-            new = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
-            dx, ddt, dA, dB, dC, dD, dz, dbias = (new(t) for t in (x, dt, A, Bm, Cm, D, z, dt_bias))
-            B, T, H, P = x.shape
-            ds = torch.empty(B, H, P, Bm.shape[-1], dtype=F32, device=x.device) if ctx.had_state else None
+            T, kind, dev = x.shape[1], x.dtype, x.device
+            dx, ddt = torch.empty(x.shape, dtype=kind, device=dev), torch.empty(dt.shape, dtype=kind, device=dev)
+            dB, dC = torch.empty(Bm.shape, dtype=kind, device=dev), torch.empty(Cm.shape, dtype=kind, device=dev)
+            dz = None if z is None else torch.empty(x.shape, dtype=kind, device=dev)
+            dA = torch.empty_like(A)
+            dD, dbias = None if D is None else torch.empty_like(D), None if dt_bias is None else torch.empty_like(dt_bias)
+            ds = torch.empty((x.shape[0], *x.shape[2:], Bm.shape[-1]), dtype=F32, device=dev) if ctx.had_state else None
             if T == 0:
                 for t in (dA, dD, dbias):
                     if t is not None:
@@ -159,9 +171,8 @@ class _Scan(torch.autograd.Function):
                     ds.zero_() if dafter is None else ds.copy_(dafter)
             else:
                 dy = torch.zeros_like(dx) if dy is None else _packed(dy, 2)
-                ops.ssm_scan_bwd(x, dt, A, Bm, Cm, D, z, dt_bias, v, states, dy, dx, ddt, dA, dB, dC, dD, dz, dbias, lengths=lengths,
-                                 dstate_out=_c(dafter), dstate=ds)
-        return dx, ddt, dA, dB, dC, dD, dz, dbias, ds, None, None
+                ops._ssm_scan_bwd(x, dt, A, Bm, Cm, D, z, dt_bias, v, states, dy, dx, ddt, dA, dB, dC, dD, dz, dbias, lengths, _c(dafter), ds)
+        return dx, ddt, dA, dB, dC, dD, dz, dbias, ds, None, None, None
 
 
 def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: torch.Tensor, Cm: torch.Tensor, *,
@@ -174,62 +185,65 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: torch
     zero).  `lengths` int32 [B]: sample b ends after lengths[b] tokens; behind it y is zero and nothing of the inputs counts.
     return_state=True also returns the state behind each sample's last token, fp32 (what selective_scan_step goes on from).
     A non-finite input may reach every output of its chunk of 64 tokens and everything behind it."""
-    x, z, Bm, Cm, dt = _packed(x, 2), _packed(z, 2), _packed(Bm, 2), _packed(Cm, 2), _packed(dt, 1)
-    state = _c(state)
+    sig = ops._sig("ssm_scan", x, dt, A, Bm, Cm, D, z, dt_bias, state, lengths)
+    if sig not in ops._SEEN:
+        x, z, Bm, Cm, dt, state = _packed(x, 2), _packed(z, 2), _packed(Bm, 2), _packed(Cm, 2), _packed(dt, 1), _c(state)
+        sig = None
     if _wants_grad(x, dt, A, Bm, Cm, D, z, dt_bias, state):
-        y, after = _Scan.apply(x, dt, A, Bm, Cm, D, z, dt_bias, state, lengths, return_state)
+        y, after = _Scan.apply(x, dt, A, Bm, Cm, D, z, dt_bias, state, lengths, return_state, sig)
     else:
         with _on(x):
-            y, after, _, _ = _scan_fwd(x, dt, A, Bm, Cm, D, z, dt_bias, state, lengths, return_state, False)
+            y, after, _, _ = _scan_fwd(x, dt, A, Bm, Cm, D, z, dt_bias, state, lengths, return_state, False, sig)
     return (y, after) if return_state else y
 
 
-@torch.no_grad()
 def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: torch.Tensor, Cm: torch.Tensor, state: torch.Tensor, *,
                         D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
                         dt_bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """selective_scan for one token: x, z [B,H,P], dt [B,H], Bm, Cm [B,G,N], state fp32 [B,H,P,N] (advances in place); returns
     [B,H,P].  No gradient."""
+    sig = ops._sig("ssm_scan_step", x, dt, A, Bm, Cm, D, z, dt_bias, state)
+    if sig not in ops._SEEN:
+        x, z, Bm, Cm, dt, sig = _packed(x, 2), _packed(z, 2), _packed(Bm, 2), _packed(Cm, 2), _packed(dt, 1), None
     with _on(x):
-        x, z, Bm, Cm, dt = _packed(x, 2), _packed(z, 2), _packed(Bm, 2), _packed(Cm, 2), _packed(dt, 1)
-        return ops.ssm_scan_step(x, dt, A, Bm, Cm, D, z, dt_bias, state, torch.empty(x.shape, dtype=x.dtype, device=x.device))
+        return ops.ssm_scan_step(x, dt, A, Bm, Cm, D, z, dt_bias, state, sig=sig)
 
 
 # ---- norms around a block -----------------------------------------------------------------------------------------------
-def _sandwich_fwd(residual, y, pw, pb, nw, nb, gate, scale, rms, eps, train):
-    h = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
-    n = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-    stats = torch.empty(y.numel() // max(y.shape[-1], 1), 4, dtype=F32, device=y.device) if train else None
-    if y.numel():
-        ops.sandwich_norm(residual, y, pw, pb, nw, nb, h, n, gate=gate, scale=scale, rms=rms, eps=eps, stats=stats)
-    return h, n, stats
+def _sandwich_fwd(residual, y, pw, pb, nw, nb, gate, scale, rms, eps, kind, train):
+    stats = None
+    if train:
+        stats = torch.empty((y.numel() // max(y.shape[-1], 1), 4), dtype=F32, device=y.device)
+    if y.numel() == 0:
+        return torch.empty_like(residual), torch.empty_like(y), stats
+    return (*ops.sandwich_norm(residual, y, pw, pb, nw, nb, gate=gate, scale=scale, rms=rms, eps=eps, stats=stats, kind=kind), stats)
 
 
 class _Sandwich(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, residual, y, pw, pb, nw, nb, gate, scale, rms, eps):
+    def forward(ctx, residual, y, pw, pb, nw, nb, gate, scale, rms, eps, kind):
         with _on(y):
-            h, n, stats = _sandwich_fwd(residual, y, pw, pb, nw, nb, gate, scale, rms, eps, True)
+            h, n, stats = _sandwich_fwd(residual, y, pw, pb, nw, nb, gate, scale, rms, eps, kind, True)
         ctx.save_for_backward(residual, y, pw, pb, nw, nb, gate, stats)
-        ctx.consts = (scale, rms, eps)
+        ctx.consts = (scale, rms, eps, kind)
         return h, n
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh, dn):
         residual, y, pw, pb, nw, nb, gate, stats = ctx.saved_tensors
-        scale, rms, eps = ctx.consts
         with _on(y):
-            new = lambda t: None if t is None else torch.empty_like(t)  # noqa: E731
-            dres, dy, dpw, dpb, dnw, dnb, dg = (new(t) for t in (residual, y, pw, pb, nw, nb, gate))
+            dres, dy, dpw, dnw = torch.empty_like(residual), torch.empty_like(y), torch.empty_like(pw), torch.empty_like(nw)
+            dpb, dnb = None if pb is None else torch.empty_like(pb), None if nb is None else torch.empty_like(nb)
+            dg = None if gate is None else torch.empty_like(gate)
             if y.numel():
-                ops.sandwich_norm_bwd(residual, y, pw, pb, nw, nb, stats, dh.contiguous(), dn.contiguous(), dres, dy, dpw, dpb, dnw, dnb,
-                                      gate=gate, dgate=dg, scale=scale, rms=rms, eps=eps)
+                ops._sandwich_norm_bwd(residual, y, pw, pb, nw, nb, stats, dh.contiguous(), dn.contiguous(), dres, dy, dpw, dpb, dnw, dnb, gate, dg,
+                                       *ctx.consts)
             else:
                 for t in (dpw, dpb, dnw, dnb, dg):
                     if t is not None:
                         t.zero_()
-        return dres, dy, dpw, dpb, dnw, dnb, dg, None, None, None
+        return dres, dy, dpw, dpb, dnw, dnb, dg, None, None, None, None
 
 
 def sandwich_norm(residual: torch.Tensor, y: torch.Tensor, post_weight: torch.Tensor, post_bias: Optional[torch.Tensor],
@@ -244,9 +258,10 @@ def sandwich_norm(residual: torch.Tensor, y: torch.Tensor, post_weight: torch.Te
         raise ValueError(f"sandwich_norm: kind {kind!r} ('layer' or 'rms')")
     if kind == "rms" and (post_bias is not None or pre_bias is not None):
         raise ValueError("sandwich_norm: kind 'rms' has no biases")
-    args = (_c(residual), _c(y), post_weight, post_bias, pre_weight, pre_bias, _c(gate), float(scale), kind == "rms", float(eps))
-    ops._sandwich_shapes("sandwich_norm", args[0], args[1], args[6], *args[2:6])
-    if _wants_grad(*args[:7]):
+    residual, y, gate = residual.contiguous(), y.contiguous(), _c(gate)
+    gate_kind = ops._sandwich_kind("sandwich_norm", residual, y, gate, post_weight, post_bias, pre_weight, pre_bias)
+    args = (residual, y, post_weight, post_bias, pre_weight, pre_bias, gate, float(scale), kind == "rms", float(eps), gate_kind)
+    if _wants_grad(residual, y, post_weight, post_bias, pre_weight, pre_bias, gate):
         return _Sandwich.apply(*args)
     with _on(y):
         return _sandwich_fwd(*args, False)[:2]
