@@ -16,7 +16,8 @@ void segments(SsmScanArgs& a) {
   a.nchunks = (a.T + SSM_CHUNK - 1) / SSM_CHUNK;
   const long rows = (long)a.B * a.H * a.pblocks;
   long n = rows >= 512 ? 1 : 512 / rows;
-  if (n > a.nchunks / 4) n = a.nchunks / 4;
+  if (n > a.nchunks / 2) n = a.nchunks / 2;      // two chunks at least: a shorter one is not worth its join
+  if (a.nchunks < 8) n = 1;                      // nor are three launches for one short walk
   if (n < 1) n = 1;
   a.seg_chunks = n == 1 ? a.nchunks : (int)((a.nchunks + n - 1) / n);
   a.nseg = a.seg_chunks ? (a.nchunks + a.seg_chunks - 1) / a.seg_chunks : 1;
@@ -168,7 +169,7 @@ int conv_args(SsmConvArgs& a, int dtype, const void* x, int64_t sxb, int64_t sxt
   RVIT_CHECK_ARG(x && w, "ssm_conv: null pointer");
   a.x = x; a.sxb = sxb; a.sxt = sxt; a.w = w; a.bias = bias; a.B = B; a.T = T; a.C = C; a.K = K; a.silu = silu;
   const int V = 16 / es(dtype);
-  a.vec = at(x, 16) && sxb % V == 0 && sxt % V == 0 && C % V == 0;
+  a.vec = at(x, 16) && at(w, 16) && at(bias, 16) && sxb % V == 0 && sxt % V == 0 && C % V == 0;
   return RVIT_OK;
 }
 // tokens of a thread: long strips reread less, short ones fill the chip
@@ -255,7 +256,7 @@ int sandwich_args(SandwichArgs& a, const void* res, int res_dtype, const void* y
   return RVIT_OK;
 }
 void sandwich_parts(SandwichArgs& a) {
-  const int want = 512;      // two workgroups per compute unit
+  const int want = 1024;      // four workgroups per compute unit
   if (a.gate_kind == 2) {
     const int64_t samples = a.rows / a.T;
     int64_t per = (want + samples - 1) / samples;

@@ -24,18 +24,30 @@ __device__ __forceinline__ void stv(T* p, const float (&v)[V]) {
   else ssm_st4(p, v);
 }
 
-// sum over the threads of a row; buf: one float per wave, two sets used in turn
+__device__ __forceinline__ float wave_total(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ssm_scan64(v)), 63)); }
+// sums over the threads of a row (WPR waves; the 4 / WPR rows of a workgroup call it together); buf: 2 x 4 x 2 floats, two sets
+// used in turn
 template <int WPR>
-__device__ __forceinline__ float row_sum(float v, float* buf, int& turn) {
-  v = wave_sum(v);
-  if constexpr (WPR == 1) return v;
-  float* s = buf + (turn ^= 1) * WPR;
-  if ((threadIdx.x & 63) == 0) s[(threadIdx.x >> 6) % WPR] = v;
-  __syncthreads();
-  v = s[0];
+__device__ __forceinline__ void row_sums(float& u, float& v, float* buf, int& turn) {
+  u = wave_total(u);
+  v = wave_total(v);
+  if constexpr (WPR > 1) {
+    float* s = buf + (turn ^= 1) * 8;
+    const int w = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) { s[w] = u; s[4 + w] = v; }
+    __syncthreads();
+    s += w / WPR * WPR;
+    u = s[0];
+    v = s[4];
 #pragma unroll
-  for (int i = 1; i < WPR; ++i) v += s[i];
-  return v;
+    for (int i = 1; i < WPR; ++i) { u += s[i]; v += s[4 + i]; }
+  }
+}
+template <int WPR>
+__device__ __forceinline__ float row_sum(float u, float* buf, int& turn) {
+  float none = 0.f;
+  row_sums<WPR>(u, none, buf, turn);
+  return u;
 }
 
 template <typename TY, int V>
@@ -52,11 +64,12 @@ __device__ __forceinline__ void ld_gate(const SandwichArgs& a, long row, int e, 
 
 template <typename TR, typename TY, int V, int WPR, int IT>
 __global__ __launch_bounds__(256) void sandwich_fwd_kernel(SandwichArgs a) {
-  __shared__ float buf[2 * WPR];
+  __shared__ float buf[16];
   int turn = 0;
   const int lid = threadIdx.x % (64 * WPR);
   const long row = (long)blockIdx.x * (4 / WPR) + threadIdx.x / (64 * WPR);
-  if (row >= a.rows) return;     // whole waves; with WPR = 4 the whole workgroup
+  static_assert(WPR == 1 || WPR == 4, "a row that does not exist ends whole workgroups, or waves that meet no barrier");
+  if (row >= a.rows) return;
   const float inv = 1.0f / a.E;
   float y[IT][V], s = 0.f;
 #pragma unroll
@@ -129,10 +142,22 @@ __global__ __launch_bounds__(256) void sandwich_fwd_kernel(SandwichArgs a) {
 
 // One workgroup per part of the rows; the columns' sums (dw1, db1, dw2, db2, dgate) stay in registers over its rows and leave
 // as part[part][5][E], added in order by sandwich_sum_kernel: no atomics.
+template <typename T, int V> struct Raw;
+template <typename T> struct Raw<T, 4> : SsmRaw4<T> {};
+template <typename T> struct Raw<T, 1> {
+  T u;
+  __device__ __forceinline__ void load(const T* p) { u = *p; }
+  __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = (float)u; }
+};
+
+// The weights (and a gate per channel or sample) are in LDS, the next row's four inputs on their way in registers while a row is
+// worked on.
 template <typename TR, typename TY, int V, int WPR, int IT>
-__global__ __launch_bounds__(256) void sandwich_bwd_kernel(SandwichArgs a) {
-  __shared__ float buf[2 * WPR];
-  __shared__ float red[WPR == 1 ? 4 * 64 * IT * V : 1];
+__global__ __launch_bounds__(256, IT * V > 4 ? 2 : 4) void sandwich_bwd_kernel(SandwichArgs a) {
+  constexpr int W = 64 * WPR * IT * V;        // columns, padded
+  __shared__ float buf[16];
+  __shared__ __attribute__((aligned(16))) float sm[4 * W];      // weight and bias behind the block, weight before the next, scale x gate
+  float *sw1 = sm, *sb1 = sm + W, *sw2 = sm + 2 * W, *sgt = sm + 3 * W;
   int turn = 0;
   constexpr int GROUPS = 4 / WPR;
   const int lid = threadIdx.x % (64 * WPR), grp = threadIdx.x / (64 * WPR);
@@ -146,6 +171,16 @@ __global__ __launch_bounds__(256) void sandwich_bwd_kernel(SandwichArgs a) {
     r0 = (long)part * a.part_rows;
     r1 = min(r0 + a.part_rows, a.rows);
   }
+  for (int e = threadIdx.x; e < W; e += 256) {
+    const bool ok = e < a.E;
+    float g[1];
+    ld_gate<TY, 1>(a, a.gate_kind == 2 ? r0 : 0, e, ok && a.gate_kind != 3, g);
+    sw1[e] = ok ? a.w1[e] : 0.f;
+    sb1[e] = ok && a.b1 ? a.b1[e] : 0.f;
+    sw2[e] = ok ? a.w2[e] : 0.f;
+    sgt[e] = g[0] * a.scale;
+  }
+  __syncthreads();
   const float inv = 1.0f / a.E;
   float acc[5][IT][V];
 #pragma unroll
@@ -154,27 +189,55 @@ __global__ __launch_bounds__(256) void sandwich_bwd_kernel(SandwichArgs a) {
     for (int it = 0; it < IT; ++it)
 #pragma unroll
       for (int j = 0; j < V; ++j) acc[k][it][j] = 0.f;
-  for (long row = r0 + grp; row < r1; row += GROUPS) {
-    const float4 st = *reinterpret_cast<const float4*>(a.stats + 4 * row);
+  Raw<TY, V> ny[IT], nn[IT];
+  Raw<TR, V> nr[IT], nh[IT];
+  float4 nst;
+  auto fetch = [&](long row) {
+    nst = *reinterpret_cast<const float4*>(a.stats + 4 * row);
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
+      const int e = (it * 64 * WPR + lid) * V;
+      const long o = row * a.E + (e < a.E ? e : 0);      // (columns outside: any address of the row, dropped below)
+      ny[it].load((const TY*)a.y + o);
+      nr[it].load((const TR*)a.res + o);
+      nn[it].load((const TY*)a.dn + o);
+      nh[it].load((const TR*)a.dh + o);
+    }
+  };
+  fetch(min(r0 + grp, r1 - 1));
+  // (all rows of the workgroup take every turn: they meet in the sums.  One that is past the end counts as zero.)
+  for (long base = r0; base < r1; base += GROUPS) {
+    const long row = base + grp;
+    const bool act = row < r1;
+    // (the lane number anew for every row: the compiler would keep the weights of all its columns in registers)
+    int lid = threadIdx.x % (64 * WPR);
+    asm volatile("" : "+v"(lid));
+    const float4 st = nst;
     float y[IT][V], d[IT][V], hh[IT][V], s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
       const int e = (it * 64 * WPR + lid) * V;
-      const bool ok = e < a.E;
+      const bool ok = e < a.E && act;
       float w1[V], b1[V], w2[V], g[V], dn[V];
-      ldv<TY, V>((const TY*)a.y + row * a.E + e, ok, y[it]);
-      ldv<TR, V>((const TR*)a.res + row * a.E + e, ok, hh[it]);
-      ldv<TY, V>((const TY*)a.dn + row * a.E + e, ok, dn);
-      ldv<TR, V>((const TR*)a.dh + row * a.E + e, ok, d[it]);
-      ldv<float, V>(a.w1 + e, ok, w1);
-      ldv<float, V>(a.b1 + e, ok && a.b1, b1);
-      ldv<float, V>(a.w2 + e, ok, w2);
-      ld_gate<TY, V>(a, row, e, ok, g);
+      ny[it].get(y[it]);
+      nr[it].get(hh[it]);
+      nn[it].get(dn);
+      nh[it].get(d[it]);
+      ldv<float, V>(sw1 + e, true, w1);
+      ldv<float, V>(sb1 + e, true, b1);
+      ldv<float, V>(sw2 + e, true, w2);
+      ldv<float, V>(sgt + e, true, g);
+      if (a.gate_kind == 3) {
+        ld_gate<TY, V>(a, row, e, ok, g);
+#pragma unroll
+        for (int j = 0; j < V; ++j) g[j] *= a.scale;
+      }
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         y[it][j] = ok ? (y[it][j] - st.x) * st.y : 0.f;                           // normalised y
-        const float h = fmaf(a.scale * g[j], fmaf(y[it][j], w1[j], b1[j]), hh[it][j]);
+        const float h = fmaf(g[j], fmaf(y[it][j], w1[j], b1[j]), hh[it][j]);
         hh[it][j] = ok ? (h - st.z) * st.w : 0.f;                                 // normalised h
+        dn[j] = ok ? dn[j] : 0.f;
         acc[2][it][j] = fmaf(dn[j], hh[it][j], acc[2][it][j]);
         acc[3][it][j] += dn[j];
         const float p = dn[j] * w2[j];
@@ -183,24 +246,31 @@ __global__ __launch_bounds__(256) void sandwich_bwd_kernel(SandwichArgs a) {
         d[it][j] = fmaf(p, st.w, d[it][j]);
       }
     }
-    s1 = a.rms ? 0.f : row_sum<WPR>(s1, buf, turn) * inv;
-    s2 = row_sum<WPR>(s2, buf, turn) * inv;
+    if (base + GROUPS < r1) fetch(min(row + GROUPS, r1 - 1));
+    row_sums<WPR>(s1, s2, buf, turn);
+    s1 = a.rms ? 0.f : s1 * inv;
+    s2 *= inv;
     float t1 = 0.f, t2 = 0.f;
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
       const int e = (it * 64 * WPR + lid) * V;
-      const bool ok = e < a.E;
+      const bool ok = e < a.E && act;
       float w1[V], b1[V], g[V], dg[V];
-      ldv<float, V>(a.w1 + e, ok, w1);
-      ldv<float, V>(a.b1 + e, ok && a.b1, b1);
-      ld_gate<TY, V>(a, row, e, ok, g);
+      ldv<float, V>(sw1 + e, true, w1);
+      ldv<float, V>(sb1 + e, true, b1);
+      ldv<float, V>(sgt + e, true, g);
+      if (a.gate_kind == 3) {
+        ld_gate<TY, V>(a, row, e, ok, g);
+#pragma unroll
+        for (int j = 0; j < V; ++j) g[j] *= a.scale;
+      }
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         d[it][j] -= st.w * (s1 + hh[it][j] * s2);                                 // dh'
-        const float sd = ok ? a.scale * d[it][j] : 0.f;
-        dg[j] = sd * fmaf(y[it][j], w1[j], b1[j]);
+        const float dh = ok ? d[it][j] : 0.f;
+        dg[j] = a.scale * dh * fmaf(y[it][j], w1[j], b1[j]);
         acc[4][it][j] += dg[j];
-        const float du = sd * g[j];
+        const float du = dh * g[j];
         acc[0][it][j] = fmaf(du, y[it][j], acc[0][it][j]);
         acc[1][it][j] += du;
         hh[it][j] = du * w1[j];
@@ -215,31 +285,33 @@ __global__ __launch_bounds__(256) void sandwich_bwd_kernel(SandwichArgs a) {
         }
       }
     }
-    t1 = a.rms ? 0.f : row_sum<WPR>(t1, buf, turn) * inv;
-    t2 = row_sum<WPR>(t2, buf, turn) * inv;
+    row_sums<WPR>(t1, t2, buf, turn);
+    t1 = a.rms ? 0.f : t1 * inv;
+    t2 *= inv;
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
       const int e = (it * 64 * WPR + lid) * V;
       float o[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) o[j] = st.y * (hh[it][j] - t1 - y[it][j] * t2);
-      if (e < a.E) stv<TY, V>((TY*)a.dy + row * a.E + e, o);
+      if (e < a.E && act) stv<TY, V>((TY*)a.dy + row * a.E + e, o);
     }
   }
   float* out = a.part + (long)part * 5 * a.E;
 #pragma unroll
   for (int k = 0; k < 5; ++k) {
     if (k == 4 && (a.gate_kind == 0 || a.gate_kind == 3)) break;
-    if constexpr (WPR == 1) {
+    if constexpr (WPR < 4) {      // the groups' sums, through the weights' LDS
       __syncthreads();
 #pragma unroll
       for (int it = 0; it < IT; ++it)
 #pragma unroll
-        for (int j = 0; j < V; ++j) red[grp * 64 * IT * V + (it * 64 + lid) * V + j] = acc[k][it][j];
+        for (int j = 0; j < V; ++j) sm[grp * W + (it * 64 * WPR + lid) * V + j] = acc[k][it][j];
       __syncthreads();
       for (int e = threadIdx.x; e < a.E; e += 256) {
-        constexpr int W = 64 * IT * V;
-        out[(long)k * a.E + e] = (red[e] + red[W + e]) + (red[2 * W + e] + red[3 * W + e]);
+        float v = sm[e] + sm[W + e];
+        if (GROUPS == 4) v += sm[2 * W + e] + sm[3 * W + e];
+        out[(long)k * a.E + e] = v;
       }
     } else {
 #pragma unroll
@@ -257,8 +329,15 @@ __global__ __launch_bounds__(1024) void sandwich_sum_kernel(SandwichArgs a, int 
   const int cx = threadIdx.x & 63, py = threadIdx.x >> 6;
   const int k = blockIdx.y, e = blockIdx.x * 64 + cx;
   double v = 0.0;
-  if (e < a.E)
-    for (int p = py; p < a.parts; p += 16) v += (double)a.part[((long)p * 5 + k) * a.E + e];
+  if (e < a.E) {
+    const long n = 5L * a.E, o = (long)k * a.E + e;
+    int p = py;
+    for (; p + 48 < a.parts; p += 64) {      // four loads on their way
+      const float u = a.part[p * n + o], w = a.part[(p + 16) * n + o], x = a.part[(p + 32) * n + o], y = a.part[(p + 48) * n + o];
+      v += ((double)u + (double)w) + ((double)x + (double)y);
+    }
+    for (; p < a.parts; p += 16) v += (double)a.part[p * n + o];
+  }
   red[py][cx] = v;
   __syncthreads();
   if (py == 0 && e < a.E) {
@@ -280,40 +359,58 @@ __global__ __launch_bounds__(256) void sandwich_sample_kernel(SandwichArgs a, in
 }
 
 template <typename TR, typename TY, int V, int WPR, int IT>
-int launch(const SandwichArgs& a, bool bwd, hipStream_t st) {
-  if (bwd) {
-    hipLaunchKernelGGL((sandwich_bwd_kernel<TR, TY, V, WPR, IT>), dim3(a.parts), dim3(256), 0, st, a);
-    RVIT_CHECK_LAUNCH("sandwich_bwd");
-    const int gb = a.gate_f32 ? 0 : (int)(sizeof(TY) == 2);
-    hipLaunchKernelGGL(sandwich_sum_kernel, dim3((a.E + 63) / 64, a.gate_kind == 1 ? 5 : 4), dim3(1024), 0, st, a, gb);
-    RVIT_CHECK_LAUNCH("sandwich_sum");
-    if (a.gate_kind == 2) {
-      const long n = a.rows / a.T * a.E;
-      hipLaunchKernelGGL(sandwich_sample_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a, gb);
-      RVIT_CHECK_LAUNCH("sandwich_sample");
-    }
-    return RVIT_OK;
+int launch_bwd(const SandwichArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((sandwich_bwd_kernel<TR, TY, V, WPR, IT>), dim3(a.parts), dim3(256), 0, st, a);
+  RVIT_CHECK_LAUNCH("sandwich_bwd");
+  const int gb = a.gate_f32 ? 0 : (int)(sizeof(TY) == 2);
+  hipLaunchKernelGGL(sandwich_sum_kernel, dim3((a.E + 63) / 64, a.gate_kind == 1 ? 5 : 4), dim3(1024), 0, st, a, gb);
+  RVIT_CHECK_LAUNCH("sandwich_sum");
+  if (a.gate_kind == 2) {
+    const long n = a.rows / a.T * a.E;
+    hipLaunchKernelGGL(sandwich_sample_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a, gb);
+    RVIT_CHECK_LAUNCH("sandwich_sample");
   }
+  return RVIT_OK;
+}
+template <typename TR, typename TY, int V, int WPR, int IT>
+int launch_fwd(const SandwichArgs& a, hipStream_t st) {
   constexpr int R = 4 / WPR;
   hipLaunchKernelGGL((sandwich_fwd_kernel<TR, TY, V, WPR, IT>), dim3((unsigned)((a.rows + R - 1) / R)), dim3(256), 0, st, a);
   RVIT_CHECK_LAUNCH("sandwich_fwd");
   return RVIT_OK;
 }
 
+// Columns of a thread.  Forward: a wave takes a row of up to 1024 columns, which meets no barrier (64 us at 25216 x 1024, what
+// its bytes take).  Backward: a thread keeps five sums a column over all rows, so few columns and more waves to a row.
 template <typename TR, typename TY>
 int launch_e(const SandwichArgs& a, bool bwd, hipStream_t st) {
-  if (a.vec) {
-    if (a.E <= 256) return launch<TR, TY, 4, 1, 1>(a, bwd, st);
-    if (a.E <= 512) return launch<TR, TY, 4, 1, 2>(a, bwd, st);
-    if (a.E <= 1024) return launch<TR, TY, 4, 1, 4>(a, bwd, st);
-    if (a.E <= 2048) return launch<TR, TY, 4, 4, 2>(a, bwd, st);
-    return launch<TR, TY, 4, 4, 4>(a, bwd, st);
+  const int E = a.E;
+  if (a.vec && !bwd) {
+    if (E <= 256) return launch_fwd<TR, TY, 4, 1, 1>(a, st);
+    if (E <= 512) return launch_fwd<TR, TY, 4, 1, 2>(a, st);
+    if (E <= 1024) return launch_fwd<TR, TY, 4, 1, 4>(a, st);
+    if (E <= 2048) return launch_fwd<TR, TY, 4, 4, 2>(a, st);
+    return launch_fwd<TR, TY, 4, 4, 4>(a, st);
   }
-  if (a.E <= 256) return launch<TR, TY, 1, 1, 4>(a, bwd, st);
-  if (a.E <= 512) return launch<TR, TY, 1, 4, 2>(a, bwd, st);
-  if (a.E <= 1024) return launch<TR, TY, 1, 4, 4>(a, bwd, st);
-  if (a.E <= 2048) return launch<TR, TY, 1, 4, 8>(a, bwd, st);
-  return launch<TR, TY, 1, 4, 16>(a, bwd, st);
+  if (a.vec) {
+    if (E <= 256) return launch_bwd<TR, TY, 4, 1, 1>(a, st);
+    if (E <= 512) return launch_bwd<TR, TY, 4, 2, 1>(a, st);
+    if (E <= 1024) return launch_bwd<TR, TY, 4, 4, 1>(a, st);
+    if (E <= 2048) return launch_bwd<TR, TY, 4, 4, 2>(a, st);
+    return launch_bwd<TR, TY, 4, 4, 4>(a, st);
+  }
+  if (!bwd) {
+    if (E <= 256) return launch_fwd<TR, TY, 1, 1, 4>(a, st);
+    if (E <= 512) return launch_fwd<TR, TY, 1, 4, 2>(a, st);
+    if (E <= 1024) return launch_fwd<TR, TY, 1, 4, 4>(a, st);
+    if (E <= 2048) return launch_fwd<TR, TY, 1, 4, 8>(a, st);
+    return launch_fwd<TR, TY, 1, 4, 16>(a, st);
+  }
+  if (E <= 256) return launch_bwd<TR, TY, 1, 1, 4>(a, st);
+  if (E <= 512) return launch_bwd<TR, TY, 1, 4, 2>(a, st);
+  if (E <= 1024) return launch_bwd<TR, TY, 1, 4, 4>(a, st);
+  if (E <= 2048) return launch_bwd<TR, TY, 1, 4, 8>(a, st);
+  return launch_bwd<TR, TY, 1, 4, 16>(a, st);
 }
 
 int go(const SandwichArgs& a, int rd, int d, bool bwd, hipStream_t st) {

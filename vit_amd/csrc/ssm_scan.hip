@@ -299,12 +299,21 @@ __global__ __launch_bounds__(256) void ssm_join_kernel(float* seg_state, const d
   const int k = i % NP, p = i / NP % P64;
   const long bh = i / ((long)NP * P64);
   float run = init && p < P && k < N ? init[(bh * P + p) * N + k] : 0.f;
-  for (int j = 0; j < nseg; ++j) {
-    const int s = reverse ? nseg - 1 - j : j;
-    const float own = seg_state[s * n + i];
-    const float f = ssm_exp2((float)seg_decay[s * BH + bh]);
-    seg_state[s * n + i] = run;
-    run = f * run + own;
+  for (int j0 = 0; j0 < nseg; j0 += 8) {      // eight loads on their way
+    float own[8], f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int m = min(j0 + j, nseg - 1), s = reverse ? nseg - 1 - m : m;
+      own[j] = seg_state[s * n + i];
+      f[j] = (float)seg_decay[s * BH + bh];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j0 + j >= nseg) break;
+      const int s = reverse ? nseg - 1 - (j0 + j) : j0 + j;
+      seg_state[s * n + i] = run;
+      run = ssm_exp2(f[j]) * run + own[j];
+    }
   }
 }
 
