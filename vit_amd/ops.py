@@ -1597,426 +1597,3 @@ def preprocess_u8_static(frames: torch.Tensor, tables_h, tables_v, resized: int,
                 _ptr(tables_v[1]), tables_v[0], resized, _ptr(crop_tl), S, float(noise_std),
                 int(noise_seed) & ((1 << 64) - 1), _ptr(out), _stream()), "rvit_preprocess_u8_static")
     return out
-
-
-# =================================================================================================
-# state-space sequence operators (csrc/ssm_conv.hip, ssm_scan.hip, ssm_scan_bwd.hip, sandwich.hip); the user-level
-# functions, with autograd, are in vit_amd/ssm.py
-# =================================================================================================
-def _f32_or_none(t: Optional[torch.Tensor], shape, what: str) -> None:
-    if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous()):
-        raise ValueError(f"{what} must be contiguous float32 {list(shape)}, got {t.dtype} {list(t.shape)}")
-
-
-def _like_or_none(t: Optional[torch.Tensor], dtype, shape, what: str) -> None:
-    if t is not None and (t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous()):
-        raise ValueError(f"{what} must be contiguous {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
-
-
-def _lengths(lengths: Optional[torch.Tensor], B: int, what: str) -> None:
-    if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,) or not lengths.is_contiguous()):
-        raise ValueError(f"{what}: lengths must be contiguous int32 [{B}], got {lengths.dtype} {list(lengths.shape)}")
-
-
-def _one_gpu(what: str, *ts: Optional[torch.Tensor]) -> None:
-    """Every tensor on one GPU."""
-    dev = ts[0].device
-    for t in ts:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
-    if dev.type != "cuda":
-        raise RuntimeError("vit_amd ops run only on the GPU (HIP); got a CPU tensor. There is no CPU fallback.")
-
-
-# These operators are also called one token at a time, where checking ten tensors costs more than the kernel: a call whose
-# operands have the shapes, strides, types and device of an earlier one that passed is not checked again.
-_SEEN: set = set()
-_SEEN_MAX = 4096
-
-
-def _sig(what: str, *ts: Optional[torch.Tensor]) -> tuple:
-    return (what, *[None if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in ts])
-
-
-def _passed(sig: tuple) -> None:
-    if len(_SEEN) >= _SEEN_MAX:
-        _SEEN.clear()
-    _SEEN.add(sig)
-
-
-def _here(what: str, t: torch.Tensor) -> None:
-    """The launch goes to the current device's stream."""
-    if t.get_device() != _raw_device():
-        raise RuntimeError(f"{what}: the tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-
-
-def _call(name: str, span: str, flops: int, nbytes, *args) -> None:
-    """One entry point on the current stream; `nbytes`: a function, called only under the profiler."""
-    if _PROF is None:
-        check(getattr(_lib.load(), name)(*args, _stream()), name)
-    else:
-        with _Span(span, flops, nbytes()):
-            check(getattr(_lib.load(), name)(*args, _stream()), name)
-
-
-def _conv_shapes(what, x, w, bias, step):
-    if x.dim() != (2 if step else 3) or x.dtype not in (BF16, torch.float32):
-        raise ValueError(f"{what}: x must be bf16 / f32 {'[B,C]' if step else '[B,T,C]'}, got {x.dtype} {list(x.shape)}")
-    if x.stride(-1) != 1 and x.shape[-1] != 1:
-        raise ValueError(f"{what}: the channels of x must be packed")
-    C = x.shape[-1]
-    if w.dim() != 2 or w.shape[0] != C or not 2 <= w.shape[1] <= 6 or x.shape[0] < 1 or C < 1:
-        raise ValueError(f"{what}: weight must be [C={C}, 2..6], got {list(w.shape)}")
-    _f32_or_none(w, w.shape, f"{what}: weight")
-    _f32_or_none(bias, (C,), f"{what}: bias")
-    return C, w.shape[1]
-
-
-def ssm_conv(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], out: torch.Tensor, *, silu: bool,
-             state: Optional[torch.Tensor] = None, state_out: Optional[torch.Tensor] = None,
-             lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """out = act(bias + causal window of x): x bf16/f32 [B,T,C] (channels packed), w f32 [C,K], out [B,T,C]; state / state_out
-    [B,K-1,C]: the inputs before the first / behind the last token of each sample."""
-    sig = _sig("ssm_conv", x, w, bias, out, state, state_out, lengths)
-    if sig not in _SEEN:
-        C, K = _conv_shapes("ssm_conv", x, w, bias, False)
-        _like_or_none(out, x.dtype, x.shape, "ssm_conv: out")
-        for t in (state, state_out):
-            _like_or_none(t, x.dtype, (x.shape[0], K - 1, C), "ssm_conv: state")
-        _lengths(lengths, x.shape[0], "ssm_conv")
-        _one_gpu("ssm_conv", x, w, bias, out, state, state_out, lengths)
-        _passed(sig)
-    _here("ssm_conv", x)
-    B, T, C = x.shape
-    K = w.shape[1]
-    sb, st, _ = x.stride()
-    _call("rvit_ssm_conv_fwd", "ssm_conv_fwd", 2 * B * T * C * K, lambda: _nbytes(x, out), x.data_ptr(), sb, st, w.data_ptr(), _ptr(bias),
-          _ptr(state), _ptr(lengths), out.data_ptr(), _ptr(state_out), _dt(x), B, T, C, K, silu)
-    return out
-
-
-@functools.lru_cache(maxsize=512)
-def _conv_bwd_bytes(B: int, T: int, C: int, K: int) -> int:
-    nb = ctypes.c_int64(0)
-    check(_lib.load().rvit_ssm_conv_bwd_workspace(ctypes.byref(nb), B, T, C, K), "rvit_ssm_conv_bwd_workspace")
-    return nb.value
-
-
-def ssm_conv_bwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], dy: torch.Tensor, dx: torch.Tensor,
-                 dw: torch.Tensor, dbias: Optional[torch.Tensor], *, silu: bool, state: Optional[torch.Tensor] = None,
-                 lengths: Optional[torch.Tensor] = None, dstate_out: Optional[torch.Tensor] = None,
-                 dstate: Optional[torch.Tensor] = None) -> None:
-    """Gradients of ssm_conv (written, not added): dx [B,T,C], dw f32 [C,K], dbias f32 [C], dstate [B,K-1,C]."""
-    sig = _sig("ssm_conv_bwd", x, w, bias, dy, dx, dw, dbias, state, lengths, dstate_out, dstate)
-    if sig not in _SEEN:
-        C, K = _conv_shapes("ssm_conv_bwd", x, w, bias, False)
-        if dy.shape != x.shape or dy.dtype != x.dtype or (dy.stride(-1) != 1 and C != 1):
-            raise ValueError("ssm_conv_bwd: dy must match x, channels packed")
-        _like_or_none(dx, x.dtype, x.shape, "ssm_conv_bwd: dx")
-        for t in (state, dstate_out, dstate):
-            _like_or_none(t, x.dtype, (x.shape[0], K - 1, C), "ssm_conv_bwd: state")
-        _f32_or_none(dw, (C, K), "ssm_conv_bwd: dw")
-        _f32_or_none(dbias, (C,), "ssm_conv_bwd: dbias")
-        _lengths(lengths, x.shape[0], "ssm_conv_bwd")
-        _one_gpu("ssm_conv_bwd", x, w, bias, dy, dx, dw, dbias, state, lengths, dstate_out, dstate)
-        _passed(sig)
-    _here("ssm_conv_bwd", x)
-    _ssm_conv_bwd(x, w, bias, dy, dx, dw, dbias, silu, state, lengths, dstate_out, dstate)
-
-
-def _ssm_conv_bwd(x, w, bias, dy, dx, dw, dbias, silu, state, lengths, dstate_out, dstate) -> None:
-    """ssm_conv_bwd for operands known to fit: a forward's checked inputs and what was allocated like them."""
-    B, T, C = x.shape
-    K = w.shape[1]
-    nb = _conv_bwd_bytes(B, T, C, K)
-    ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
-    sb, st, _ = x.stride()
-    yb, yt, _ = dy.stride()
-    _call("rvit_ssm_conv_bwd", "ssm_conv_bwd", 4 * B * T * C * K, lambda: _nbytes(x, dy, dx), x.data_ptr(), sb, st, w.data_ptr(), _ptr(bias),
-          _ptr(state), _ptr(lengths), dy.data_ptr(), yb, yt, _ptr(dstate_out), dx.data_ptr(), dw.data_ptr(), _ptr(dbias), _ptr(dstate),
-          ws.data_ptr(), nb, _dt(x), B, T, C, K, silu)
-
-
-def ssm_conv_step(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], state: torch.Tensor,
-                  out: Optional[torch.Tensor] = None, *, silu: bool, sig: Optional[tuple] = None) -> torch.Tensor:
-    """One token: x [B,C], out [B,C]; state [B,K-1,C] advances in place.  sig: _sig("ssm_conv_step", x, w, bias, state)."""
-    if sig is None:
-        sig = _sig("ssm_conv_step", x, w, bias, state)
-    if sig not in _SEEN:
-        C, K = _conv_shapes("ssm_conv_step", x, w, bias, True)
-        _like_or_none(state, x.dtype, (x.shape[0], K - 1, C), "ssm_conv_step: state")
-        _one_gpu("ssm_conv_step", x, w, bias, state)
-        _passed(sig)
-    _here("ssm_conv_step", x)
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    else:
-        _like_or_none(out, x.dtype, x.shape, "ssm_conv_step: out")
-        _one_gpu("ssm_conv_step", x, out)
-    B, C = x.shape
-    K = w.shape[1]
-    _call("rvit_ssm_conv_step", "ssm_conv_step", 2 * B * C * K, lambda: _nbytes(x, out, state, state), x.data_ptr(), x.stride(0), w.data_ptr(),
-          _ptr(bias), state.data_ptr(), out.data_ptr(), _dt(x), B, C, K, silu)
-    return out
-
-
-SSM_MAX_STATE = 128
-
-
-def _scan_shapes(what, x, dt, A, Bm, Cm, D, z, dt_bias, step):
-    lead = 1 if step else 2
-    if x.dim() != lead + 2 or x.dtype not in (BF16, torch.float32):
-        raise ValueError(f"{what}: x must be bf16 / f32 {'[B,H,P]' if step else '[B,T,H,P]'}, got {x.dtype} {list(x.shape)}")
-    H, P = x.shape[-2:]
-    if Bm.dim() != lead + 2 or Bm.shape != Cm.shape or Bm.shape[:lead] != x.shape[:lead]:
-        raise ValueError(f"{what}: Bm and Cm must be {'[B,G,N]' if step else '[B,T,G,N]'}, got {list(Bm.shape)} and {list(Cm.shape)}")
-    G, N = Bm.shape[-2:]
-    if min(x.shape[0], H, P, G, N) < 1 or H % G or N > SSM_MAX_STATE:
-        raise ValueError(f"{what}: {H} heads in {G} groups, {P} channels, {N} states (at most {SSM_MAX_STATE})")
-    if dt.shape != x.shape[:lead + 1]:
-        raise ValueError(f"{what}: dt must be {list(x.shape[:lead + 1])}, got {list(dt.shape)}")
-    if z is not None and z.shape != x.shape:
-        raise ValueError(f"{what}: z must be {list(x.shape)}, got {list(z.shape)}")
-    for t, inner in ((x, 2), (Bm, 2), (Cm, 2), (z, 2), (dt, 1)):
-        if t is None:
-            continue
-        if t.dtype != x.dtype:
-            raise ValueError(f"{what}: x, dt, Bm, Cm, z of one dtype, got {x.dtype} and {t.dtype}")
-        if (t.stride(-1) != 1 and t.shape[-1] != 1) or (inner == 2 and t.stride(-2) != t.shape[-1] and t.shape[-2] != 1):
-            raise ValueError(f"{what}: heads and channels of a token must be packed, got strides {t.stride()}")
-    for t, n in ((A, "A"), (D, "D"), (dt_bias, "dt_bias")):
-        _f32_or_none(t, (H,), f"{what}: {n}")
-    return H, P, G, N
-
-
-def _ts(t: Optional[torch.Tensor]):
-    return (None, 0, 0) if t is None else (t.data_ptr(), *t.stride()[:2])
-
-
-@functools.lru_cache(maxsize=512)
-def ssm_scan_plan(B: int, T: int, H: int, P: int, G: int, N: int) -> Tuple[int, int, int]:
-    """(workspace bytes of the forward, floats of the kept chunk states, workspace bytes of the backward)."""
-    v = [ctypes.c_int64(0) for _ in range(3)]
-    check(_lib.load().rvit_ssm_scan_plan(*[ctypes.byref(i) for i in v], B, T, H, P, G, N), "rvit_ssm_scan_plan")
-    return tuple(i.value for i in v)
-
-
-def ssm_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: torch.Tensor, Cm: torch.Tensor, D: Optional[torch.Tensor],
-             z: Optional[torch.Tensor], dt_bias: Optional[torch.Tensor], out: Optional[torch.Tensor] = None, *,
-             state: Optional[torch.Tensor] = None, state_out: Optional[torch.Tensor] = None,
-             lengths: Optional[torch.Tensor] = None, v: Optional[torch.Tensor] = None,
-             states: Optional[torch.Tensor] = None, sig: Optional[tuple] = None) -> torch.Tensor:
-    """Selective scan over [B,T]: x, z, out [B,T,H,P], dt [B,T,H], Bm, Cm [B,T,G,N], A, D, dt_bias f32 [H], state / state_out
-    f32 [B,H,P,N].  Training passes v (like out; with z) and states (f32, ssm_scan_plan()[1] values) for the backward.
-    sig: _sig("ssm_scan", x, dt, A, Bm, Cm, D, z, dt_bias, state, lengths)."""
-    if sig is None:
-        sig = _sig("ssm_scan", x, dt, A, Bm, Cm, D, z, dt_bias, state, lengths)
-    if sig not in _SEEN:
-        H, P, G, N = _scan_shapes("ssm_scan", x, dt, A, Bm, Cm, D, z, dt_bias, False)
-        _f32_or_none(state, (x.shape[0], H, P, N), "ssm_scan: state")
-        _lengths(lengths, x.shape[0], "ssm_scan")
-        _one_gpu("ssm_scan", x, dt, A, Bm, Cm, D, z, dt_bias, state, lengths)
-        _passed(sig)
-    _here("ssm_scan", x)
-    B, T, H, P = x.shape
-    G, N = Bm.shape[2:]
-    fwd_bytes, state_floats, _ = ssm_scan_plan(B, T, H, P, G, N)
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    else:
-        _like_or_none(out, x.dtype, x.shape, "ssm_scan: out")
-        _one_gpu("ssm_scan", x, out)
-    if v is not None or states is not None or state_out is not None:
-        _like_or_none(v, x.dtype, x.shape, "ssm_scan: v")
-        _f32_or_none(states, (state_floats,), "ssm_scan: states")
-        _f32_or_none(state_out, (B, H, P, N), "ssm_scan: state_out")
-        _one_gpu("ssm_scan", x, v, states, state_out)
-    ws = torch.empty(fwd_bytes, dtype=torch.uint8, device=x.device) if fwd_bytes > 16 else None
-    _call("rvit_ssm_scan_fwd", "ssm_scan_fwd", B * T * H * P * (5 * N + 6), lambda: _nbytes(x, dt, Bm, Cm, z, out, state, state_out), *_ts(x),
-          *_ts(dt), A.data_ptr(), *_ts(Bm), *_ts(Cm), _ptr(D), *_ts(z), _ptr(dt_bias), _ptr(state), _ptr(lengths), out.data_ptr(), _ptr(v),
-          _ptr(state_out), _ptr(states), _ptr(ws), fwd_bytes, _dt(x), B, T, H, P, G, N)
-    return out
-
-
-def ssm_scan_bwd(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: torch.Tensor, Cm: torch.Tensor,
-                 D: Optional[torch.Tensor], z: Optional[torch.Tensor], dt_bias: Optional[torch.Tensor], v: Optional[torch.Tensor],
-                 states: torch.Tensor, dy: torch.Tensor, dx: torch.Tensor, ddt: torch.Tensor, dA: torch.Tensor, dB: torch.Tensor,
-                 dC: torch.Tensor, dD: Optional[torch.Tensor], dz: Optional[torch.Tensor], ddt_bias: Optional[torch.Tensor], *,
-                 lengths: Optional[torch.Tensor] = None, dstate_out: Optional[torch.Tensor] = None,
-                 dstate: Optional[torch.Tensor] = None) -> None:
-    """Gradients of ssm_scan (written, not added), each like what it belongs to; v and states are the forward's."""
-    sig = _sig("ssm_scan_bwd", x, dt, A, Bm, Cm, D, z, dt_bias, v, states, dy, dx, ddt, dA, dB, dC, dD, dz, ddt_bias, lengths, dstate_out,
-               dstate)
-    if sig not in _SEEN:
-        H, P, G, N = _scan_shapes("ssm_scan_bwd", x, dt, A, Bm, Cm, D, z, dt_bias, False)
-        B, T = x.shape[:2]
-        if dy.shape != x.shape or dy.dtype != x.dtype or (dy.stride(3) != 1 and P != 1) or (dy.stride(2) != P and H != 1):
-            raise ValueError("ssm_scan_bwd: dy must match x, heads and channels packed")
-        if (z is None) != (dz is None) or (z is not None and v is None):
-            raise ValueError("ssm_scan_bwd: z, dz and v come together")
-        for t, like in ((v, x), (dx, x), (dz, x), (ddt, dt), (dB, Bm), (dC, Cm)):
-            _like_or_none(t, x.dtype, like.shape, "ssm_scan_bwd: gradients")
-        for t in (dA, dD, ddt_bias):
-            _f32_or_none(t, (H,), "ssm_scan_bwd: dA, dD, ddt_bias")
-        for t in (dstate_out, dstate):
-            _f32_or_none(t, (B, H, P, N), "ssm_scan_bwd: dstate")
-        _lengths(lengths, B, "ssm_scan_bwd")
-        _f32_or_none(states, (ssm_scan_plan(B, T, H, P, G, N)[1],), "ssm_scan_bwd: states")
-        _one_gpu("ssm_scan_bwd", x, dt, A, Bm, Cm, D, z, dt_bias, v, states, dy, dx, ddt, dA, dB, dC, dD, dz, ddt_bias, lengths,
-                 dstate_out, dstate)
-        _passed(sig)
-    _here("ssm_scan_bwd", x)
-    _ssm_scan_bwd(x, dt, A, Bm, Cm, D, z, dt_bias, v, states, dy, dx, ddt, dA, dB, dC, dD, dz, ddt_bias, lengths, dstate_out, dstate)
-
-
-def _ssm_scan_bwd(x, dt, A, Bm, Cm, D, z, dt_bias, v, states, dy, dx, ddt, dA, dB, dC, dD, dz, ddt_bias, lengths, dstate_out, dstate) -> None:
-    """ssm_scan_bwd for operands known to fit: a forward's checked inputs and what was allocated like them."""
-    B, T, H, P = x.shape
-    G, N = Bm.shape[2:]
-    nb = ssm_scan_plan(B, T, H, P, G, N)[2]
-    ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
-    _call("rvit_ssm_scan_bwd", "ssm_scan_bwd", B * T * H * P * (10 * N + 12), lambda: _nbytes(x, dt, Bm, Cm, z, dy, dx, ddt, dB, dC, dz), *_ts(x),
-          *_ts(dt), A.data_ptr(), *_ts(Bm), *_ts(Cm), _ptr(D), *_ts(z), _ptr(dt_bias), _ptr(lengths), _ptr(v), states.data_ptr(), *_ts(dy),
-          _ptr(dstate_out), dx.data_ptr(), ddt.data_ptr(), dA.data_ptr(), dB.data_ptr(), dC.data_ptr(), _ptr(dD), _ptr(dz), _ptr(ddt_bias),
-          _ptr(dstate), ws.data_ptr(), nb, _dt(x), B, T, H, P, G, N)
-
-
-def ssm_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: torch.Tensor, Cm: torch.Tensor,
-                  D: Optional[torch.Tensor], z: Optional[torch.Tensor], dt_bias: Optional[torch.Tensor], state: torch.Tensor,
-                  out: Optional[torch.Tensor] = None, *, sig: Optional[tuple] = None) -> torch.Tensor:
-    """One token: x, z, out [B,H,P], dt [B,H], Bm, Cm [B,G,N]; state f32 [B,H,P,N] advances in place.
-    sig: _sig("ssm_scan_step", x, dt, A, Bm, Cm, D, z, dt_bias, state)."""
-    if sig is None:
-        sig = _sig("ssm_scan_step", x, dt, A, Bm, Cm, D, z, dt_bias, state)
-    if sig not in _SEEN:
-        H, P, G, N = _scan_shapes("ssm_scan_step", x, dt, A, Bm, Cm, D, z, dt_bias, True)
-        _f32_or_none(state, (x.shape[0], H, P, N), "ssm_scan_step: state")
-        _one_gpu("ssm_scan_step", x, dt, A, Bm, Cm, D, z, dt_bias, state)
-        _passed(sig)
-    _here("ssm_scan_step", x)
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    else:
-        _like_or_none(out, x.dtype, x.shape, "ssm_scan_step: out")
-        _one_gpu("ssm_scan_step", x, out)
-    B, H, P = x.shape
-    _, G, N = Bm.shape
-    _call("rvit_ssm_scan_step", "ssm_scan_step", B * H * P * (5 * N + 6), lambda: _nbytes(x, dt, Bm, Cm, z, out, state, state), x.data_ptr(),
-          x.stride(0), dt.data_ptr(), dt.stride(0), A.data_ptr(), Bm.data_ptr(), Bm.stride(0), Cm.data_ptr(), Cm.stride(0), _ptr(D), _ptr(z),
-          0 if z is None else z.stride(0), _ptr(dt_bias), state.data_ptr(), out.data_ptr(), _dt(x), B, H, P, G, N)
-    return out
-
-
-SANDWICH_MAX_E = 4096
-
-
-def _sandwich_shapes(what, residual, y, gate, pw, pb, nw, nb):
-    E = y.shape[-1]
-    for t, n in ((residual, "residual"), (y, "y")):
-        if t.dtype not in (BF16, torch.float32) or t.shape != y.shape or not t.is_contiguous():
-            raise ValueError(f"{what}: residual and y must be contiguous bf16 / f32 of one shape, got {n} {t.dtype} {list(t.shape)}")
-    if y.dim() < 2 or not 1 <= E <= SANDWICH_MAX_E:
-        raise ValueError(f"{what}: y must be [..., E] with E <= {SANDWICH_MAX_E}, got {list(y.shape)}")
-    for t, n in ((pw, "post weight"), (pb, "post bias"), (nw, "pre weight"), (nb, "pre bias")):
-        _f32_or_none(t, (E,), f"{what}: {n}")
-    if gate is None:
-        return E, 0
-    if gate.dtype not in (torch.float32, y.dtype) or not gate.is_contiguous():
-        raise ValueError(f"{what}: gate must be contiguous float32 or {y.dtype}, got {gate.dtype}")
-    if gate.shape == y.shape[-1:]:
-        return E, 1
-    if gate.shape == y.shape:
-        return E, 3
-    if y.dim() == 3 and gate.shape == (y.shape[0], E):
-        return E, 2
-    raise ValueError(f"{what}: gate must be [E], [B,E] (with y [B,T,E]) or like y {list(y.shape)}, got {list(gate.shape)}")
-
-
-_SANDWICH_KIND: dict = {}      # signature that passed -> gate kind
-
-
-def _sandwich_kind(what, residual, y, gate, pw, pb, nw, nb) -> int:
-    sig = _sig(what, residual, y, gate, pw, pb, nw, nb)
-    kind = _SANDWICH_KIND.get(sig)
-    if kind is None:
-        kind = _sandwich_shapes(what, residual, y, gate, pw, pb, nw, nb)[1]
-        _one_gpu(what, residual, y, gate, pw, pb, nw, nb)
-        if len(_SANDWICH_KIND) >= _SEEN_MAX:
-            _SANDWICH_KIND.clear()
-        _SANDWICH_KIND[sig] = kind
-    return kind
-
-
-def sandwich_norm(residual: torch.Tensor, y: torch.Tensor, post_w: torch.Tensor, post_b: Optional[torch.Tensor], pre_w: torch.Tensor,
-                  pre_b: Optional[torch.Tensor], h: Optional[torch.Tensor] = None, n: Optional[torch.Tensor] = None, *,
-                  gate: Optional[torch.Tensor] = None, scale: float = 1.0, rms: bool = False, eps: float = 1e-5,
-                  stats: Optional[torch.Tensor] = None, kind: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
-    """h = residual + scale * gate * norm_post(y), n = norm_pre(h); [..., E], h like residual, n like y; stats f32 [rows,4]
-    (for the backward).  kind: _sandwich_kind of the operands."""
-    if kind is None:
-        kind = _sandwich_kind("sandwich_norm", residual, y, gate, post_w, post_b, pre_w, pre_b)
-    _here("sandwich_norm", y)
-    E = y.shape[-1]
-    rows = y.numel() // E
-    if h is None:
-        h = torch.empty_like(residual)
-    else:
-        _like_or_none(h, residual.dtype, y.shape, "sandwich_norm: h")
-    if n is None:
-        n = torch.empty_like(y)
-    else:
-        _like_or_none(n, y.dtype, y.shape, "sandwich_norm: n")
-    if stats is not None:
-        _f32_or_none(stats, (rows, 4), "sandwich_norm: stats")
-        _one_gpu("sandwich_norm", y, h, n, stats)
-    _call("rvit_sandwich_norm_fwd", "sandwich_norm_fwd", 20 * rows * E, lambda: _nbytes(residual, y, h, n), residual.data_ptr(), _dt(residual),
-          y.data_ptr(), _dt(y), _ptr(gate), kind, RVIT_F32 if gate is None else _dt(gate), scale, post_w.data_ptr(), _ptr(post_b),
-          pre_w.data_ptr(), _ptr(pre_b), eps, rms, h.data_ptr(), n.data_ptr(), _ptr(stats), rows, y.shape[-2], E)
-    return h, n
-
-
-@functools.lru_cache(maxsize=512)
-def _sandwich_bwd_bytes(rows: int, T: int, E: int, kind: int) -> int:
-    nb = ctypes.c_int64(0)
-    check(_lib.load().rvit_sandwich_norm_bwd_workspace(ctypes.byref(nb), rows, T, E, kind), "rvit_sandwich_norm_bwd_workspace")
-    return nb.value
-
-
-def sandwich_norm_bwd(residual: torch.Tensor, y: torch.Tensor, post_w: torch.Tensor, post_b: Optional[torch.Tensor], pre_w: torch.Tensor,
-                      pre_b: Optional[torch.Tensor], stats: torch.Tensor, dh: torch.Tensor, dn: torch.Tensor, dresidual: torch.Tensor,
-                      dy: torch.Tensor, dpost_w: torch.Tensor, dpost_b: Optional[torch.Tensor], dpre_w: torch.Tensor,
-                      dpre_b: Optional[torch.Tensor], *, gate: Optional[torch.Tensor] = None, dgate: Optional[torch.Tensor] = None,
-                      scale: float = 1.0, rms: bool = False, eps: float = 1e-5) -> None:
-    """Gradients of sandwich_norm (written, not added), each like what it belongs to."""
-    kind = _sandwich_kind("sandwich_norm_bwd", residual, y, gate, post_w, post_b, pre_w, pre_b)
-    _here("sandwich_norm_bwd", y)
-    E = y.shape[-1]
-    rows = y.numel() // E
-    sig = _sig("sandwich_norm_bwd", residual, y, gate, stats, dh, dn, dresidual, dy, dpost_w, dpost_b, dpre_w, dpre_b, dgate)
-    if sig not in _SEEN:
-        for t, like in ((dh, residual), (dresidual, residual), (dn, y), (dy, y)):
-            _like_or_none(t, like.dtype, y.shape, "sandwich_norm_bwd: gradients")
-        if (gate is None) != (dgate is None):
-            raise ValueError("sandwich_norm_bwd: gate and dgate come together")
-        if gate is not None:
-            _like_or_none(dgate, gate.dtype, gate.shape, "sandwich_norm_bwd: dgate")
-        for t in (dpost_w, dpost_b, dpre_w, dpre_b):
-            _f32_or_none(t, (E,), "sandwich_norm_bwd: parameter gradients")
-        _f32_or_none(stats, (rows, 4), "sandwich_norm_bwd: stats")
-        _one_gpu("sandwich_norm_bwd", y, stats, dh, dn, dresidual, dy, dpost_w, dpost_b, dpre_w, dpre_b, dgate)
-        _passed(sig)
-    _sandwich_norm_bwd(residual, y, post_w, post_b, pre_w, pre_b, stats, dh, dn, dresidual, dy, dpost_w, dpost_b, dpre_w, dpre_b, gate, dgate,
-                       scale, rms, eps, kind)
-
-
-def _sandwich_norm_bwd(residual, y, post_w, post_b, pre_w, pre_b, stats, dh, dn, dresidual, dy, dpost_w, dpost_b, dpre_w, dpre_b, gate, dgate,
-                       scale, rms, eps, kind) -> None:
-    """sandwich_norm_bwd for operands known to fit: a forward's checked inputs and what was allocated like them."""
-    E = y.shape[-1]
-    rows = y.numel() // E
-    nb = _sandwich_bwd_bytes(rows, y.shape[-2], E, kind)
-    ws = torch.empty(nb, dtype=torch.uint8, device=y.device)
-    _call("rvit_sandwich_norm_bwd", "sandwich_norm_bwd", 45 * rows * E, lambda: _nbytes(residual, y, dh, dn, dresidual, dy), residual.data_ptr(),
-          _dt(residual), y.data_ptr(), _dt(y), _ptr(gate), kind, RVIT_F32 if gate is None else _dt(gate), scale, post_w.data_ptr(), _ptr(post_b),
-          pre_w.data_ptr(), _ptr(pre_b), eps, rms, stats.data_ptr(), dh.data_ptr(), dn.data_ptr(), dresidual.data_ptr(), dy.data_ptr(),
-          _ptr(dgate), dpost_w.data_ptr(), _ptr(dpost_b), dpre_w.data_ptr(), _ptr(dpre_b), ws.data_ptr(), nb, rows, y.shape[-2], E)
