@@ -324,3 +324,215 @@ def test_captured_steps_replay(dev):
         assert torch.equal(out, want) and torch.equal(conv, c2) and torch.equal(state, s2)
         assert torch.equal(out2, _call(ssm, long))
         torch.cuda.synchronize()
+
+
+def _scan_case(seed, dtype, dev, B, T, H, P, G, N, **kw):
+    """CPU inputs and their 64-bit outputs and gradients (cotangent: every output), and the device copy as leaves."""
+    s = scan_inputs(seed, dtype, B, T, H, P, G, N, **kw)
+    names = [k for k in SCAN_NAMES if s[k] is not None]
+    dy = randn(torch.Generator().manual_seed(seed), B, T, H, P, dtype=dtype)
+    leaf = leaves64(s)
+    wy, _ = ref.selective_scan(**leaf)
+    want = torch.autograd.grad(wy, [leaf[k] for k in names], dy.double())
+    return s, names, dy, wy, dict(zip(names, want)), {k: v if v is None else v.requires_grad_() for k, v in to(s, dev).items()}
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_token_strides_past_32_bits(dev, dtype):
+    """Each of x, z, Bm, Cm, dt and dy alone with tokens 2^25 elements apart (70 of them: byte offsets past 2^32)."""
+    from vit_amd import ssm
+    T, H, P, N = 70, 2, 32, 32
+    s, names, dy, wy, want, d = _scan_case(40, DTYPES[dtype], dev, 1, T, H, P, 1, N)
+    far = torch.empty((T - 1) * 2 ** 25 + H * P, dtype=DTYPES[dtype], device=dev)
+
+    def spread(v):
+        inner = v[0, 0].numel()
+        out = far.as_strided((1, T, inner), (far.numel(), 2 ** 25, 1)).unflatten(-1, v.shape[2:])
+        return out.copy_(v.detach())
+
+    for k in ("x", "z", "Bm", "Cm", "dt", "dy"):
+        c = dict(d)
+        if k != "dy":
+            c[k] = spread(d[k]).requires_grad_()
+        y = _call(ssm, c)
+        close("y " + k, y, wy)
+        got = torch.autograd.grad(y, [c[n] for n in names], spread(dy.to(dev)) if k == "dy" else dy.to(dev))
+        for n, a in zip(names, got):
+            close(f"d{n}, {k} far", a, want[n])
+
+
+def test_expanded_gradient(dev):
+    """A sum's gradient is one element spread out: strides of zero."""
+    from vit_amd import ssm
+    s, names, _, wy, _, d = _scan_case(41, torch.float32, dev, 2, 100, 2, 16, 1, 16)
+    leaf = leaves64(s)
+    want = torch.autograd.grad(ref.selective_scan(**leaf)[0].sum(), [leaf[k] for k in names])
+    for k, a, b in zip(names, torch.autograd.grad(_call(ssm, d).sum(), [d[k] for k in names]), want):
+        close("d" + k, a, b)
+    x, w = randn(torch.Generator().manual_seed(1), 2, 9, 8), randn(torch.Generator().manual_seed(2), 8, 4)
+    lx, lw = x.double().requires_grad_(), w.double().requires_grad_()
+    want = torch.autograd.grad(ref.causal_conv(lx, lw)[0].sum(), [lx, lw])
+    gx, gw = x.to(dev).requires_grad_(), w.to(dev).requires_grad_()
+    for a, b in zip(torch.autograd.grad(ssm.causal_conv(gx, gw).sum(), [gx, gw]), want):
+        close("d", a, b)
+
+
+def test_steps_near_the_types_end(dev):
+    """A step of 1e37 (a decay whose logarithm is outside fp32, two in one chunk) forgets what came before, and no more."""
+    from vit_amd import ssm
+    s = scan_inputs(42, torch.float32, 1, 100, 2, 16, 1, 16, state=True)
+    s["A"].fill_(-16.0)
+    for t in (30, 40, 80):
+        s["dt"][:, t] = 1e37
+        s["x"][:, t] *= 1e-34
+    leaf = leaves64(s)
+    wy, wend = ref.selective_scan(**leaf)
+    dy = randn(torch.Generator().manual_seed(5), *wy.shape)
+    want = torch.autograd.grad(wy, [leaf[k] for k in ("Bm", "Cm", "z", "state")], dy.double())
+    d = {k: v.requires_grad_() for k, v in to(s, dev).items()}
+    y, end = _call(ssm, d, return_state=True)
+    for a, b in ((0, 30), (30, 31), (31, 40), (40, 41), (41, 60), (60, 80), (80, 100)):
+        close(f"y {a}..{b}", y[:, a:b], wy[:, a:b])
+    close("end", end, wend)
+    for k, a, b in zip(("Bm", "Cm", "z", "state"), torch.autograd.grad(y, [d[k] for k in ("Bm", "Cm", "z", "state")], dy.to(dev)), want):
+        close("d" + k, a, b)
+
+
+def test_second_derivatives_are_refused(dev):
+    from vit_amd import ssm
+    s = {k: v.requires_grad_() for k, v in to(scan_inputs(43, torch.float32, 1, 5, 1, 4, 1, 4, state=True), dev).items()}
+    x, w, e = s["x"].flatten(2), torch.ones(4, 4, device=dev, requires_grad=True), torch.ones(4, device=dev, requires_grad=True)
+    for out, leaf in ((_call(ssm, s), s["x"]), (ssm.causal_conv(x, w), w), (ssm.sandwich_norm(x, x, e, None, e, None)[1], e)):
+        with pytest.raises(RuntimeError, match="second derivatives"):
+            torch.autograd.grad(out.sum(), leaf, create_graph=True)
+
+
+def test_a_graph_notices_a_state_that_moved_on(dev):
+    """The convolution's backward pass reads the kept inputs it started from; a step on them in between is an error, not a wrong
+    gradient."""
+    from vit_amd import ssm
+    x, w, st = torch.randn(2, 5, 8, device=dev), torch.randn(8, 4, device=dev, requires_grad=True), torch.randn(2, 3, 8, device=dev)
+    y = ssm.causal_conv(x, w, state=st)
+    ssm.causal_conv_step(x[:, 0], w.detach(), None, st)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    s = to(scan_inputs(44, torch.float32, 2, None, 2, 8, 1, 8, state=True), dev)
+    before = s["state"]._version
+    ssm.selective_scan_step(s["x"], s["dt"], s["A"], s["Bm"], s["Cm"], s["state"])
+    assert s["state"]._version == before + 1
+    with torch.inference_mode():
+        ssm.selective_scan_step(s["x"], s["dt"], s["A"], s["Bm"], s["Cm"], s["state"].clone())
+
+
+def test_large_batches_of_short_samples(dev):
+    """More samples than a grid's second dimension holds, forward and backward."""
+    from vit_amd import ssm
+    B, T, C, E = 70000, 2, 4, 8
+    g = torch.Generator().manual_seed(45)
+    x, w, dy = randn(g, B, T, C), randn(g, C, 3), randn(g, B, T, C)
+    lx, lw = x.double().requires_grad_(), w.double().requires_grad_()
+    wy, _ = ref.causal_conv(lx, lw, silu=True)
+    want = torch.autograd.grad(wy, [lx, lw], dy.double())
+    gx, gw = x.to(dev).requires_grad_(), w.to(dev).requires_grad_()
+    y = ssm.causal_conv(gx, gw, activation="silu")
+    close("y", y, wy)
+    for a, b in zip(torch.autograd.grad(y, [gx, gw], dy.to(dev)), want):
+        close("d", a, b)
+    s, names, dy, wy, want, d = _scan_case(46, torch.float32, dev, B, 1, 1, 2, 1, 2, state=True)
+    y = _call(ssm, d)
+    close("y", y, wy)
+    for k, a in zip(names, torch.autograd.grad(y, [d[k] for k in names], dy.to(dev))):
+        close("d" + k, a, want[k])
+    for T in (1, 2):          # a gate per sample
+        s = dict(residual=randn(g, B, T, E), y=randn(g, B, T, E), post_weight=randn(g, E), post_bias=None, pre_weight=randn(g, E), pre_bias=None,
+                 gate=randn(g, B, E))
+        dn = randn(g, B, T, E)
+        leaf = leaves64(s)
+        _, wn = ref.sandwich_norm(**leaf)
+        names = [k for k in s if s[k] is not None]
+        want = torch.autograd.grad(wn, [leaf[k] for k in names], dn.double())
+        d = {k: v if v is None else v.to(dev).requires_grad_() for k, v in s.items()}
+        n = ssm.sandwich_norm(**d)[1]
+        close("n", n, wn)
+        for k, a, b in zip(names, torch.autograd.grad(n, [d[k] for k in names], dn.to(dev)), want):
+            close("d" + k, a, b)
+
+
+def test_two_streams_at_once(dev):
+    """Two long calls in flight on two streams, forward and backward, each with its own workspace."""
+    from vit_amd import ssm
+    cases = [to(scan_inputs(50 + i, torch.bfloat16, 2, 2000, 4, 64, 1, 128), dev) for i in range(2)]
+    names = [k for k in SCAN_NAMES if cases[0][k] is not None]
+    leaves = [{k: v if v is None else v.requires_grad_() for k, v in s.items()} for s in cases]
+    dy = torch.randn(2, 2000, 4, 64, device=dev).bfloat16()
+
+    def run(s):
+        y = _call(ssm, s)
+        return [y.detach()] + list(torch.autograd.grad(y, [s[k] for k in names], dy))
+
+    alone = [run(s) for s in leaves]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in leaves]
+    both = []
+    for s, st in zip(leaves, streams):
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            both.append(run(s))
+    torch.cuda.synchronize()
+    for a, b in zip(alone, both):
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_captured_training_step_replays(dev, dtype):
+    """Convolution, scan (cut into segments) and norms with their backward passes in one captured graph, replayed with new
+    inputs and eager work between, against eager calls."""
+    from vit_amd import ssm
+    B, T, H, P, N = 1, 600, 2, 32, 32
+    W = H * P + 2 * N
+    dt = DTYPES[dtype]
+    g = torch.Generator().manual_seed(60)
+    raw = randn(g, B, T, W, dtype=dt).to(dev).requires_grad_()
+    rest = to(scan_inputs(61, dt, B, T, H, P, 1, N), dev)
+    par = dict(w=randn(g, W, 4, scale=0.5), b=randn(g, W, scale=0.1), pw=randn(g, H * P, shift=1.0), nw=randn(g, H * P, shift=1.0), gate=randn(g, B, H * P))
+    par = {k: v.to(dev).requires_grad_() for k, v in par.items()}
+    leaves = [raw, *par.values()] + [rest[k].requires_grad_() for k in ("A", "D", "dt_bias")]
+    res = randn(g, B, T, H * P).to(dev)
+    cot = randn(g, B, T, H * P, dtype=dt).to(dev)
+
+    def step():
+        u = ssm.causal_conv(raw, par["w"], par["b"], activation="silu")
+        x, Bm, Cm = u[..., :H * P].unflatten(-1, (H, P)), u[..., H * P:H * P + N].unflatten(-1, (1, N)), u[..., H * P + N:].unflatten(-1, (1, N))
+        y = ssm.selective_scan(x, rest["dt"], rest["A"], Bm, Cm, D=rest["D"], z=rest["z"], dt_bias=rest["dt_bias"])
+        n = ssm.sandwich_norm(res, y.flatten(2), par["pw"], None, par["nw"], None, gate=par["gate"], kind="rms")[1]
+        return [n.detach()] + list(torch.autograd.grad(n, leaves, cot))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(4):
+        with torch.no_grad():
+            raw.copy_(randn(g, B, T, W, dtype=dt))
+        cot.copy_(randn(g, B, T, H * P, dtype=dt))
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_mixed_devices_are_refused(dev):
+    from vit_amd import ssm
+    s = to(scan_inputs(70, torch.float32, 1, 5, 1, 4, 1, 4), dev)
+    for k in ("A", "Bm", "z"):
+        with pytest.raises(ValueError, match="cpu"):
+            _call(ssm, dict(s, **{k: s[k].cpu()}))
+    with pytest.raises(ValueError, match="cpu"):
+        ssm.causal_conv(torch.zeros(1, 4, 4, device=dev), torch.zeros(4, 4))
+    with pytest.raises(ValueError, match="cpu"):
+        ssm.sandwich_norm(torch.zeros(3, 8, device=dev), torch.zeros(3, 8), torch.ones(8, device=dev), None, torch.ones(8, device=dev), None)

@@ -8,6 +8,9 @@ namespace {
 
 bool at(const void* p, unsigned a) { return (((uintptr_t)p) & (a - 1)) == 0; }
 int es(int dtype) { return dtype == RVIT_BF16 ? 2 : 4; }
+// Token strides under this fit a 32-bit byte offset over the tokens of a chunk, which the kernels' wide paths use (63 strides
+// of fp32 and a row's columns: 63 * 4 * (2^24 - 1) + 4 * 128 < 2^32); larger ones take the paths with 64-bit offsets.
+constexpr int64_t MOST = 1 << 24;
 
 // Segments of a sequence.  One workgroup walks a (sample, head, 64 channels), and a compute unit holds two of them; where there
 // are too few to fill the chip the sequence is cut, at the price of a pass that only computes states.
@@ -56,10 +59,9 @@ int inputs(SsmScanArgs& a, int dtype, const void* x, int64_t sxb, int64_t sxt, c
   a.x = x; a.dt = dt; a.A = A; a.Bm = Bm; a.Cm = Cm; a.D = D; a.z = z; a.dt_bias = dt_bias; a.lengths = lengths;
   a.sxb = sxb; a.sxt = sxt; a.sdb = sdb; a.sdt = sdt; a.sbb = sbb; a.sbt = sbt; a.scb = scb; a.sct = sct; a.szb = szb; a.szt = szt;
   const int V = 16 / es(dtype);
-  const int64_t most = 1 << 24;       // token strides that fit a 32-bit offset over the tokens of a chunk
-  a.vec_x = at(x, 16) && sxt < most && sbt < most && sct < most && sxb % V == 0 && sxt % V == 0 && a.P % V == 0;
+  a.vec_x = at(x, 16) && sxt < MOST && sbt < MOST && sct < MOST && (int64_t)a.H * a.P < MOST && sxb % V == 0 && sxt % V == 0 && a.P % V == 0;
   a.vec_bc = at(Bm, 16) && at(Cm, 16) && sbb % V == 0 && sbt % V == 0 && scb % V == 0 && sct % V == 0 && a.N % V == 0;
-  a.vec_z = at(z, 4 * es(dtype)) && szb % 4 == 0 && szt % 4 == 0 && a.P % 4 == 0;
+  a.vec_z = at(z, 4 * es(dtype)) && szt < MOST && szb % 4 == 0 && szt % 4 == 0 && a.P % 4 == 0;
   return RVIT_OK;
 }
 
@@ -128,7 +130,7 @@ int rvit_ssm_scan_bwd(const void* x, int64_t sxb, int64_t sxt, const void* dt, i
   a.f.vec_y = at(v, 4 * es(dtype)) && P % 4 == 0;
   a.f.vec_state = N % 4 == 0 && at(dstate_out, 16) && at(dstate0, 16);
   RVIT_CHECK_ARG(at(states, 16), "ssm_scan_bwd: states alignment");
-  a.vec_dy = at(dy, 4 * es(dtype)) && syb % 4 == 0 && syt % 4 == 0 && P % 4 == 0;
+  a.vec_dy = at(dy, 4 * es(dtype)) && syt < MOST && syb % 4 == 0 && syt % 4 == 0 && P % 4 == 0;
   a.vec_out = at(dx, 4 * es(dtype)) && at(dz, 4 * es(dtype)) && P % 4 == 0;
   a.vec_dbc = at(dB, 4 * es(dtype)) && at(dC, 4 * es(dtype)) && N % 4 == 0;
   char* ws = (char*)workspace;
@@ -183,7 +185,6 @@ void strips(SsmConvArgs& a, int dtype) {
 void bwd_strips(int& strip, int& n, int64_t B, int64_t T, int64_t C) {
   int64_t s = 32;
   while (s > 4 && B * ((T + 8 * s - 1) / (8 * s)) * ((C + 255) / 256) < 512) s /= 2;
-  while (B * ((T + 8 * s - 1) / (8 * s)) > 65535) s *= 2;
   strip = (int)s;
   n = (int)((T + s - 1) / s);
 }
@@ -218,7 +219,6 @@ int rvit_ssm_conv_bwd(const void* x, int64_t sxb, int64_t sxt, const float* w, c
   if (int e = conv_args(a, dtype, x, sxb, sxt, w, bias, B, T, C, K, silu)) return e;
   int64_t need = 0;
   if (int e = rvit_ssm_conv_bwd_workspace(&need, B, T, C, K)) return e;
-  RVIT_CHECK_ARG(B <= 65535, "ssm_conv_bwd: batch of %d", B);
   RVIT_CHECK_ARG(dy && dx && dw && workspace && at(workspace, 16) && workspace_bytes >= need, "ssm_conv_bwd: null pointer, or workspace of %lld bytes, %lld needed",
                  (long long)workspace_bytes, (long long)need);
   a.state = state; a.lengths = lengths; a.dy = dy; a.syb = syb; a.syt = syt; a.dstate_out = dstate_out; a.dx = dx; a.dw = dw; a.dbias = dbias;

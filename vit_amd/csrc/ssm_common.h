@@ -300,6 +300,12 @@ __device__ __forceinline__ float ssm_softplus(float x) {
   p = fmaf(p, u, 1.0f);
   return x != x ? x : fmaxf(x, 0.f) + 2.0f * s * p;
 }
+// log2 of a token's decay exp(d A), in 64 bits (A2 = A log2 e).  Held to -1e5, which is a decay of zero as well: steps of 1e37
+// would give sums outside fp32, and the difference of two infinite ones is no decay.
+__device__ __forceinline__ double ssm_log_decay(float d, double A2) {
+  const double l = (double)d * A2;
+  return l < -1e5 ? -1e5 : l;
+}
 
 // A ROWS x COLS image on its way from global memory (row stride `ld`) to LDS through the registers of a workgroup: load() is
 // issued a chunk ahead of store(), so that its latency passes under the products between.  What lies outside rows x cols is

@@ -136,9 +136,10 @@ __global__ __launch_bounds__(256, 4) void ssm_conv_bwd_kernel(SsmConvArgs a) {
   __shared__ float red[8][32][V];
   const int groups = a.C / V;
   const int gx = threadIdx.x & 31, sy = threadIdx.x >> 5;
-  const int cg = blockIdx.x * 32 + gx;
+  const int cblocks = (groups + 31) / 32, cx = blockIdx.x % cblocks, pi = blockIdx.x / cblocks;
+  const int cg = cx * 32 + gx;
   const int sblocks = (a.strips + 7) / 8;
-  const int b = blockIdx.y / sblocks, s = (blockIdx.y % sblocks) * 8 + sy;
+  const int b = pi / sblocks, s = (pi % sblocks) * 8 + sy;
   float dw[K][V], db[V];
 #pragma unroll
   for (int k = 0; k < K; ++k) zero<V>(dw[k]);
@@ -216,7 +217,7 @@ __global__ __launch_bounds__(256, 4) void ssm_conv_bwd_kernel(SsmConvArgs a) {
     }
   }
   // [part][K + 1][C]
-  float* part = a.part + (long)blockIdx.y * (K + 1) * a.C;
+  float* part = a.part + (long)pi * (K + 1) * a.C;
 #pragma unroll
   for (int k = 0; k <= K; ++k) {
     __syncthreads();
@@ -227,7 +228,7 @@ __global__ __launch_bounds__(256, 4) void ssm_conv_bwd_kernel(SsmConvArgs a) {
       float v = 0.f;
 #pragma unroll
       for (int y = 0; y < 8; ++y) v += red[y][i / V][i % V];
-      const int c = blockIdx.x * 32 * V + i;
+      const int c = cx * 32 * V + i;
       if (c < a.C) part[(long)k * a.C + c] = v;
     }
   }
@@ -289,7 +290,7 @@ int launch(const SsmConvArgs& a, int what, hipStream_t st) {
   const int groups = a.C / V;
   if (what == SSM_CONV_BWD) {
     const int sblocks = (a.strips + 7) / 8;
-    hipLaunchKernelGGL((ssm_conv_bwd_kernel<T, V, K>), dim3((groups + 31) / 32, a.B * sblocks), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((ssm_conv_bwd_kernel<T, V, K>), dim3((unsigned)((groups + 31) / 32) * (a.B * sblocks)), dim3(256), 0, st, a);
     RVIT_CHECK_LAUNCH("ssm_conv_bwd");
     hipLaunchKernelGGL(ssm_conv_sum_kernel, dim3((unsigned)(((long)(K + 1) * a.C + 63) / 64)), dim3(1024), 0, st, a.part, a.dw, a.dbias, a.B * sblocks, a.C, K);
     RVIT_CHECK_LAUNCH("ssm_conv_sum");

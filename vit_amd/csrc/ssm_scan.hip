@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_
   auto decay = [&](T raw, int ch) {
     float* sd = decays + (ch & 1) * 5 * Q;
     const float d = ch * Q + lane < len ? ssm_softplus((float)raw + bias) : 0.f;
-    const double l2 = ssm_scan64((double)d * A2), end = ssm_last_lane(l2);
+    const double l2 = ssm_scan64(ssm_log_decay(d, A2)), end = ssm_last_lane(l2);
     const float hi = (float)l2;
     sd[lane] = d;
     sd[Q + lane] = hi;
@@ -325,7 +325,7 @@ __global__ __launch_bounds__(256) void ssm_scan_step_kernel(SsmStepArgs a) {
   const int h = id % a.H, b = id / a.H;
   const int g = h / (a.H / a.G);
   const float d = ssm_softplus(ssm_ld((const T*)a.dt + b * a.sdb + h) + (a.dt_bias ? a.dt_bias[h] : 0.f));
-  const float f = ssm_exp2((float)((double)d * ((double)a.A[h] * 1.4426950408889634)));
+  const float f = ssm_exp2((float)ssm_log_decay(d, (double)a.A[h] * 1.4426950408889634));
   const T* x = (const T*)a.x + b * a.sxb + (long)h * a.P;
   const T* Bm = (const T*)a.Bm + b * a.sbb + (long)g * a.N;
   const T* Cm = (const T*)a.Cm + b * a.scb + (long)g * a.N;

@@ -76,7 +76,7 @@ __global__ __launch_bounds__(256, 2) void ssm_scan_bwd_state_kernel(SsmBwdArgs a
   auto fetch_dt = [&](int ch) { return dt[(long)min(max(ch, 0) * Q + lane, len - 1) * f.sdt]; };
   auto decay = [&](T raw, int ch) {
     const float d = ch * Q + lane < len ? ssm_softplus((float)raw + bias) : 0.f;
-    const double l2 = ssm_scan64((double)d * A2);
+    const double l2 = ssm_scan64(ssm_log_decay(d, A2));
     decays[(ch & 1) * Q + lane] = ssm_exp2((float)l2);
     total += ssm_last_lane(l2);
   };
@@ -430,7 +430,7 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
         if (w == 0) {
           const float raw = (float)rawn + (f.dt_bias ? f.dt_bias[h] : 0.f);
           const float d = lane < live ? ssm_softplus(raw) : 0.f;
-          const double l2 = ssm_scan64((double)d * ((double)Ah * 1.4426950408889634)), end = ssm_last_lane(l2);
+          const double l2 = ssm_scan64(ssm_log_decay(d, (double)Ah * 1.4426950408889634)), end = ssm_last_lane(l2);
           const float hi = (float)l2;
           sd[lane] = d;
           shi[lane] = hi;

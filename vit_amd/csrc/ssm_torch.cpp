@@ -70,6 +70,10 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
   return false;
 }
 void first_order(const char* op) { TORCH_CHECK(!at::GradMode::is_enabled(), op, ": no second derivatives (create_graph=True)"); }
+// a state that a kernel advanced in place: a graph that saved it must notice
+void advanced(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 Opt some(const Tensor& t) { return t.defined() ? Opt(t) : Opt(); }
 
 // ---- short causal convolution ----
@@ -160,6 +164,7 @@ Tensor conv_step(Tensor x, const Tensor& w, const Opt& bias_, const Tensor& stat
   done(rvit_ssm_conv_step(ptr(x), x.stride(0), w.data_ptr<float>(), (const float*)ptr(bias), ptr(state), ptr(y), dtype(x), size(x.size(0), "causal_conv_step"),
                           size(x.size(1), "causal_conv_step"), (int)w.size(1), silu, stream(x)),
        "rvit_ssm_conv_step");
+  advanced(state);
   return y;
 }
 
@@ -290,6 +295,7 @@ Tensor scan_step(Tensor x, Tensor dt, const Tensor& A, Tensor Bm, Tensor Cm, con
   done(rvit_ssm_scan_step(ptr(x), x.stride(0), ptr(dt), dt.stride(0), A.data_ptr<float>(), ptr(Bm), Bm.stride(0), ptr(Cm), Cm.stride(0), (const float*)ptr(D), ptr(z),
                           stride(z, 0), (const float*)ptr(dt_bias), (float*)ptr(state), ptr(y), dtype(x), d.B, d.H, d.P, d.G, d.N, stream(x)),
        "rvit_ssm_scan_step");
+  advanced(state);
   return y;
 }
 
@@ -311,7 +317,7 @@ int sandwich_shapes(const Tensor& residual, const Tensor& y, const Tensor& pw, c
   if (gate.sizes() == y.sizes()) return 3;
   TORCH_CHECK_VALUE(y.dim() == 3 && gate.dim() == 2 && gate.size(0) == y.size(0) && gate.size(1) == E, op, ": gate must be [E], [B,E] (with y [B,T,E]) or like y ",
                     y.sizes(), ", got ", gate.sizes());
-  return 2;
+  return y.size(1) == 1 ? 3 : 2;      // (samples of one row: the rows' own gates)
 }
 
 std::pair<Tensor, Tensor> sandwich_run(const Tensor& residual, const Tensor& y, const Tensor& pw, const Tensor& pb, const Tensor& nw, const Tensor& nb,
