@@ -67,7 +67,7 @@ __device__ __forceinline__ void scores(const T* Bs, const T* Cs, T* Gs, const fl
 // One workgroup (four waves) per (sample, head, 64 channels, segment), chunk after chunk, the state in registers: wave w
 // holds S^T for channels 16w .. 16w+15, which is the A operand of exp(L_t) S C as it lies in the accumulators.
 // A chunk's images and decays are fetched and worked out while the chunk before it is computed.
-// YOUT = false: only the state a segment reaches from zero, and the segment's summed log decay (long sequences of few
+// YOUT = false: only the state a segment (but the last) reaches from zero, and the segment's summed log decay (long sequences of few
 // rows are cut into segments, joined by ssm_join_kernel).  VEC: all wide accesses are aligned and whole.
 template <typename T, int NP, bool YOUT, bool VEC>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_scan_fwd_kernel(SsmScanArgs a) {
@@ -82,7 +82,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_
   float* decays = (float*)((T*)smem + L::END);   // two sets, by turns: d, L (high, low), exp(L_Q - L) d, exp(L)
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, q = lane >> 4, c = lane & 15;
   long id = blockIdx.x;
-  const int seg = id % a.nseg; id /= a.nseg;
+  const int segs = YOUT ? a.nseg : a.nseg - 1;     // (the last one's end is nobody's start)
+  const int seg = id % segs; id /= segs;
   const int pb = id % a.pblocks; id /= a.pblocks;
   const int h = id % a.H;
   const int b = id / a.H;
@@ -108,12 +109,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_
   f32x4 S[NT];
   const bool has_p = p0 + c < pw;
   const long srow = (((long)b * a.H + h) * a.P + pb * 64 + p0 + c) * a.N;   // row of this lane's channel in [B,H,P,N]
-  const long prow = ((((long)b * a.H + h) * a.pblocks + pb) * 64 + p0 + c) * NP;   // and in the padded copies
+  const long prow = (((long)b * a.H + h) * a.pblocks + pb) * 64 * NP + (q * 64 + p0 + c) * 4;   // and in the padded copies
   auto get_state = [&](const float* in, bool padded) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float v[4] = {0.f, 0.f, 0.f, 0.f};
-      if (padded) ssm_ld4(in + prow + 16 * nt + 4 * q, v);
+      if (padded) ssm_ld4(in + prow + 1024 * nt, v);
       else if (has_p) ssm_ld4v<VEC>(in + srow + 16 * nt + 4 * q, a.N - 16 * nt - 4 * q, v);
       S[nt] = f32x4{v[0], v[1], v[2], v[3]};
     }
@@ -122,7 +123,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const float v[4] = {S[nt][0], S[nt][1], S[nt][2], S[nt][3]};
-      if (padded) ssm_st4(out + prow + 16 * nt + 4 * q, v);
+      if (padded) ssm_st4(out + prow + 1024 * nt, v);
       else if (has_p) ssm_st4v<VEC>(out + srow + 16 * nt + 4 * q, a.N - 16 * nt - 4 * q, v);
     }
   };
@@ -292,28 +293,42 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_
 
 // Joins the segments: in place, the state a segment reached from zero becomes the state it starts from.  `reverse` runs from
 // the last segment to the first (the backward pass).  `init` [B,H,P,N] (or null) is what the first one starts from.
-__global__ __launch_bounds__(256) void ssm_join_kernel(float* seg_state, const double* seg_decay, const float* init, long n, int P, int N, int P64, int NP,
-                                                       long BH, int nseg, int reverse) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const int k = i % NP, p = i / NP % P64;
-  const long bh = i / ((long)NP * P64);
-  float run = init && p < P && k < N ? init[(bh * P + p) * N + k] : 0.f;
-  for (int j0 = 0; j0 < nseg; j0 += 8) {      // eight loads on their way
-    float own[8], f[8];
+// A thread takes four states of a channel through all segments, the next ones' on their way: its bytes in and out (192 rows of 2
+// segments, 25 MB: 6.2 us, with one state a thread 12.5; 16 rows of 32 segments, 34 MB: 13.6 and 14.6).
+__global__ __launch_bounds__(64) void ssm_join_kernel(float* seg_state, const double* seg_decay, const float* init, long n, int P, int N, int pblocks, int NP,
+                                                      long BH, int nseg, int reverse) {
+  const long i = (long)blockIdx.x * 64 + threadIdx.x;      // of the four: [BH][pblocks][NP / 4][64]
+  if (i >= n / 4) return;
+  const int p0 = i & 63, k = (int)(i >> 6) % (NP / 4) * 4;
+  const long row = i / (16 * NP), bh = row / pblocks;
+  const int p = (int)(row % pblocks) * 64 + p0;
+  f32x4 run = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int m = min(j0 + j, nseg - 1), s = reverse ? nseg - 1 - m : m;
-      own[j] = seg_state[s * n + i];
-      f[j] = (float)seg_decay[s * BH + bh];
+  for (int j = 0; j < 4; ++j) run[j] = init && p < P && k + j < N ? init[(bh * P + p) * N + k + j] : 0.f;
+  constexpr int AHEAD = 8;
+  f32x4* st = (f32x4*)seg_state + i;
+  const long step = (reverse ? -n : n) / 4;
+  const long sb = reverse ? -BH : BH;
+  const double* dec = seg_decay + (reverse ? (nseg - 1) * BH : 0) + bh;
+  if (reverse) st += (nseg - 1) * (n / 4);
+  for (int j0 = 0; j0 < nseg; j0 += AHEAD) {
+    f32x4 own[AHEAD];
+    float f[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      own[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      f[j] = 0.f;
+      if (j0 + j < nseg - 1) {      // (of the last one nothing is needed)
+        own[j] = st[(j0 + j) * step];
+        f[j] = (float)dec[(j0 + j) * sb];
+      }
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (j0 + j >= nseg) break;
-      const int s = reverse ? nseg - 1 - (j0 + j) : j0 + j;
-      seg_state[s * n + i] = run;
-      run = ssm_exp2(f[j]) * run + own[j];
-    }
+    for (int j = 0; j < AHEAD; ++j)
+      if (j0 + j < nseg) {
+        st[(j0 + j) * step] = run;
+        run = ssm_exp2(f[j]) * run + own[j];
+      }
   }
 }
 
@@ -365,7 +380,7 @@ int launch_fwd(const SsmScanArgs& a, hipStream_t st) {
   static RvitLdsLimit lim;
   constexpr int bytes = FwdLds<T, NP>::BYTES;
   if (int e = lim.ensure({(const void*)ssm_scan_fwd_kernel<T, NP, YOUT, VEC>}, bytes, "ssm_scan_fwd")) return e;
-  hipLaunchKernelGGL((ssm_scan_fwd_kernel<T, NP, YOUT, VEC>), dim3((unsigned)((long)a.B * a.H * a.pblocks * a.nseg)), dim3(256), bytes, st, a);
+  hipLaunchKernelGGL((ssm_scan_fwd_kernel<T, NP, YOUT, VEC>), dim3((unsigned)((long)a.B * a.H * a.pblocks * (YOUT ? a.nseg : a.nseg - 1))), dim3(256), bytes, st, a);
   RVIT_CHECK_LAUNCH("ssm_scan_fwd");
   return RVIT_OK;
 }
@@ -387,8 +402,8 @@ int launch_fwd_n(const SsmScanArgs& a, bool yout, hipStream_t st) {
 }  // namespace
 
 int rvit_ssm_join(float* seg_state, const double* seg_decay, const float* init, const SsmScanArgs& a, int reverse, hipStream_t st) {
-  hipLaunchKernelGGL(ssm_join_kernel, dim3((unsigned)((a.seg_stride + 255) / 256)), dim3(256), 0, st, seg_state, seg_decay, init, a.seg_stride, a.P, a.N,
-                     a.pblocks * 64, ssm_padded_n(a.N), (long)a.B * a.H, a.nseg, reverse);
+  hipLaunchKernelGGL(ssm_join_kernel, dim3((unsigned)((a.seg_stride / 4 + 63) / 64)), dim3(64), 0, st, seg_state, seg_decay, init, a.seg_stride, a.P, a.N,
+                     a.pblocks, ssm_padded_n(a.N), (long)a.B * a.H, a.nseg, reverse);
   RVIT_CHECK_LAUNCH("ssm_join");
   return RVIT_OK;
 }

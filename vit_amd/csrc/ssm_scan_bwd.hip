@@ -34,7 +34,8 @@ __global__ __launch_bounds__(256, 2) void ssm_scan_bwd_state_kernel(SsmBwdArgs a
   const SsmScanArgs& f = a.f;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, q = lane >> 4, c = lane & 15;
   long id = blockIdx.x;
-  const int seg = id % f.nseg; id /= f.nseg;
+  const int segs = OUT ? f.nseg : f.nseg - 1;      // (the first one's start is nobody's end)
+  const int seg = id % segs + (f.nseg - segs); id /= segs;
   const int pb = id % f.pblocks; id /= f.pblocks;
   const int h = id % f.H, b = id / f.H;
   const int g = h / (f.H / f.G);
@@ -50,12 +51,12 @@ __global__ __launch_bounds__(256, 2) void ssm_scan_bwd_state_kernel(SsmBwdArgs a
   f32x4 S[NT];
   const bool has_p = p0 + c < pw;
   const long srow = (((long)b * f.H + h) * f.P + pb * 64 + p0 + c) * f.N;
-  const long prow = ((((long)b * f.H + h) * f.pblocks + pb) * 64 + p0 + c) * NP;
+  const long prow = (((long)b * f.H + h) * f.pblocks + pb) * 64 * NP + (q * 64 + p0 + c) * 4;
   auto get_state = [&](const float* in, bool padded) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float v[4] = {0.f, 0.f, 0.f, 0.f};
-      if (padded) ssm_ld4(in + prow + 16 * nt + 4 * q, v);
+      if (padded) ssm_ld4(in + prow + 1024 * nt, v);
       else if (has_p) ssm_ld4v<VEC>(in + srow + 16 * nt + 4 * q, f.N - 16 * nt - 4 * q, v);
       S[nt] = f32x4{v[0], v[1], v[2], v[3]};
     }
@@ -64,7 +65,7 @@ __global__ __launch_bounds__(256, 2) void ssm_scan_bwd_state_kernel(SsmBwdArgs a
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const float v[4] = {S[nt][0], S[nt][1], S[nt][2], S[nt][3]};
-      if (padded) ssm_st4(out + prow + 16 * nt + 4 * q, v);
+      if (padded) ssm_st4(out + prow + 1024 * nt, v);
       else if (has_p) ssm_st4v<VEC>(out + srow + 16 * nt + 4 * q, f.N - 16 * nt - 4 * q, v);
     }
   };
@@ -263,7 +264,7 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
     f32x4 dsn[NP / 32];
     T rawn = (T)0.f;
     float* Ds = (float*)(smem + L::DS);
-    // (padded copies: [64 channels][NP] of a head are one piece)
+    // (padded copies: [NP / 4][64 channels][4] of a head are one piece)
     auto padded = [&](int h, int pb) { return (long)ch * f.seg_stride + (((long)b * f.H + h) * f.pblocks + pb) * 64 * NP; };
     auto fetch = [&](int h, int pb) {
       int tid = threadIdx.x;
@@ -445,14 +446,14 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
 #pragma unroll
           for (int i = 0; i < NP / 32; ++i) {
             const int e = i * 512 + tid;
-            *reinterpret_cast<f32x4*>(Ds + e / (NP / 4) * L::PS + e % (NP / 4) * 4) = dsn[i];
+            *reinterpret_cast<f32x4*>(Ds + (e & 63) * L::PS + (e >> 6) * 4) = dsn[i];
           }
         }
         const int pt = w & 3, p0 = 16 * pt;
         __builtin_amdgcn_sched_barrier(0);
         __syncthreads();
         // this wave's 16 states of S as columns (k = channels), for dC
-        const unsigned col = 8 * q * NP + 16 * nt + c;
+        const unsigned col = (4 * nt + (c >> 2)) * 256 + 32 * q + (c & 3);
         const float* dS = a.dstates + padded(h, pb);
         float sc[2][8];
         {
@@ -460,7 +461,7 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sc[ks][j] = (S0 + (32 * ks + j) * NP)[col];
+            for (int j = 0; j < 8; ++j) sc[ks][j] = (S0 + (32 * ks + j) * 4)[col];
         }
         // score tiles
 #pragma unroll
@@ -526,9 +527,9 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
             for (int k2 = 0; k2 < 2; ++k2) bf[k2] = ssm_row(Bs, PN, 16 * st[k2] + c, 32 * m + 8 * q);
             float v[8];      // dS, rows of this wave's channels
             if (L::DS_LDS || a.dstates) {
-              const float* src = L::DS_LDS ? Ds + (p0 + c) * L::PS + 32 * m + 8 * q : dS + (p0 + c) * NP + 32 * m + 8 * q;
+              const float* src = L::DS_LDS ? Ds + (p0 + c) * L::PS + 32 * m + 8 * q : dS + (8 * m + 2 * q) * 256 + (p0 + c) * 4;
               ssm_ld4(src, reinterpret_cast<float(&)[4]>(v[0]));
-              ssm_ld4(src + 4, reinterpret_cast<float(&)[4]>(v[4]));
+              ssm_ld4(src + (L::DS_LDS ? 4 : 256), reinterpret_cast<float(&)[4]>(v[4]));
             } else {
 #pragma unroll
               for (int j = 0; j < 8; ++j) v[j] = 0.f;
@@ -577,7 +578,7 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
           for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              dsc[ks][j] = L::DS_LDS ? Ds[(32 * ks + 8 * q + j) * L::PS + 16 * nt + c] : a.dstates ? (dS + (32 * ks + j) * NP)[col] : 0.f;
+              dsc[ks][j] = L::DS_LDS ? Ds[(32 * ks + 8 * q + j) * L::PS + 16 * nt + c] : a.dstates ? (dS + (32 * ks + j) * 4)[col] : 0.f;
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -709,14 +710,14 @@ int launch_bwd(const SsmBwdArgs& a, hipStream_t st) {
   if (int e = lim_o.ensure({(const void*)ssm_scan_bwd_state_kernel<T, NP, true, VEC>}, sb, "ssm_scan_bwd_state")) return e;
   if (int e = lim_s.ensure({(const void*)ssm_scan_bwd_state_kernel<T, NP, false, VEC>}, sb, "ssm_scan_bwd_state")) return e;
   if (int e = lim_c.ensure({(const void*)ssm_scan_bwd_chunk_kernel<T, NP, VEC>}, cb, "ssm_scan_bwd_chunk")) return e;
-  const dim3 grid((unsigned)((long)f.B * f.H * f.pblocks * f.nseg));
+  const long rows = (long)f.B * f.H * f.pblocks;
   if (f.nseg > 1) {
-    hipLaunchKernelGGL((ssm_scan_bwd_state_kernel<T, NP, false, VEC>), grid, dim3(256), sb, st, a);
+    hipLaunchKernelGGL((ssm_scan_bwd_state_kernel<T, NP, false, VEC>), dim3((unsigned)(rows * (f.nseg - 1))), dim3(256), sb, st, a);
     RVIT_CHECK_LAUNCH("ssm_scan_bwd_state");
     if (int e = rvit_ssm_join(f.seg_state, f.seg_decay, a.dstate_out, f, 1, st)) return e;
   }
   if (a.dstates) {
-    hipLaunchKernelGGL((ssm_scan_bwd_state_kernel<T, NP, true, VEC>), grid, dim3(256), sb, st, a);
+    hipLaunchKernelGGL((ssm_scan_bwd_state_kernel<T, NP, true, VEC>), dim3((unsigned)(rows * f.nseg)), dim3(256), sb, st, a);
     RVIT_CHECK_LAUNCH("ssm_scan_bwd_state");
   }
   hipLaunchKernelGGL((ssm_scan_bwd_chunk_kernel<T, NP, VEC>), dim3((unsigned)((long)f.B * f.nchunks * f.G * a.hsplit)), dim3(512), cb, st, a);
