@@ -22,6 +22,11 @@ namespace {
 
 constexpr int Q = SSM_CHUNK;
 
+// Everything here is linear in (v', dS), and every other chunk works on their negatives.  The matrix cores drop the low bits of
+// what they align downwards, towards minus infinity; over thousands of tokens that tilts sums whose other factors are mostly
+// of one sign (dA was 1e-6 of its size too low, for bf16 operands).  With the signs in turn the tilts cancel.
+__device__ __forceinline__ float chunk_sign(int ch) { return ch & 1 ? -1.f : 1.f; }
+
 // ---- sweep: dS before a chunk = exp(L_Q) dS behind it + sum_t exp(L_t) v'_t C_t^T ----
 template <typename T, int NP, bool OUT, bool VEC>
 __global__ __launch_bounds__(256, 2) void ssm_scan_bwd_state_kernel(SsmBwdArgs a) {
@@ -30,7 +35,7 @@ __global__ __launch_bounds__(256, 2) void ssm_scan_bwd_state_kernel(SsmBwdArgs a
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* Cs = (T*)smem;
   float* Vs = (float*)(Cs + Q * PN);
-  float* decays = Vs + Q * PV;                // two sets of exp(L_t), by turns
+  float* decays = Vs + Q * PV;                // two sets of exp(L_t) with the sign of the chunk before, by turns
   const SsmScanArgs& f = a.f;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, q = lane >> 4, c = lane & 15;
   long id = blockIdx.x;
@@ -78,7 +83,7 @@ __global__ __launch_bounds__(256, 2) void ssm_scan_bwd_state_kernel(SsmBwdArgs a
   auto decay = [&](T raw, int ch) {
     const float d = ch * Q + lane < len ? ssm_softplus((float)raw + bias) : 0.f;
     const double l2 = ssm_scan64(ssm_log_decay(d, A2));
-    decays[(ch & 1) * Q + lane] = ssm_exp2((float)l2);
+    decays[(ch & 1) * Q + lane] = chunk_sign(ch - 1) * ssm_exp2((float)l2);
     total += ssm_last_lane(l2);
   };
   const int c0 = seg * f.seg_chunks, cl = min(min(f.nchunks, c0 + f.seg_chunks), (len + Q - 1) / Q);
@@ -114,6 +119,10 @@ __global__ __launch_bounds__(256, 2) void ssm_scan_bwd_state_kernel(SsmBwdArgs a
       *reinterpret_cast<float4*>(Vs + t * PV + p) = make_float4(v[0], v[1], v[2], v[3]);
     }
   };
+  // (the state behind a chunk is held with the chunk's sign)
+  const float first = chunk_sign(max(cl, c0) - 1), last = chunk_sign(c0 - 1);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) S[nt] *= first;
   T raw = (T)0.f;
   if (c0 < cl) {
     fetch(cl - 1);
@@ -134,7 +143,7 @@ __global__ __launch_bounds__(256, 2) void ssm_scan_bwd_state_kernel(SsmBwdArgs a
       raw = fetch_dt(ch - 2);
     }
     {
-      const float eQ = se[Q - 1];
+      const float eQ = -fabsf(se[Q - 1]);
       typename O::template Cm<3> vw[2];
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
@@ -161,6 +170,8 @@ __global__ __launch_bounds__(256, 2) void ssm_scan_bwd_state_kernel(SsmBwdArgs a
       put(ch - 1);
     }
   }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) S[nt] *= last;
   if (!OUT) {
     put_state(f.seg_state + seg * f.seg_stride, true);
     if (threadIdx.x == 0 && pb == 0) f.seg_decay[((long)seg * f.B + b) * f.H + h] = total;
@@ -232,6 +243,7 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
   const int h0 = g * r + hs * a.hper, h1 = min(g * r + r, h0 + a.hper);
   const int len = f.lengths ? min(max(f.lengths[b], 0), f.T) : f.T;
   const int live = min(max(len - t0, 0), Q), here = min(f.T - t0, Q);
+  const float sign = chunk_sign(ch);
   const long ldo = (long)f.H * f.P;
   float* part = a.part + ((long)b * f.nchunks + ch) * f.H * 3;
   const int nt = w % NT, cg = w / NT;
@@ -373,10 +385,10 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
       e_u += e;
       if (pb == f.pblocks - 1) {
         const bool ok = u < live;
-        const float ddt = ok ? (e_u + f.A[h] * da_u) * ssg[u] : 0.f;
+        const float ddt = ok ? sign * (e_u + f.A[h] * da_u) * ssg[u] : 0.f;
         if (u < here) ssm_st((T*)a.ddt + ((long)b * f.T + t0 + u) * f.H + h, ddt);
-        const float sA = ssm_scan64(ok ? da_u * sd[u] : 0.f), sb = ssm_scan64(ddt);
-        if (lane == 63) { part[h * 3] = sA; part[h * 3 + 1] = dD; part[h * 3 + 2] = sb; }
+        const float sA = ssm_scan64(ok ? sign * da_u * sd[u] : 0.f), sb = ssm_scan64(ddt);
+        if (lane == 63) { part[h * 3] = sA; part[h * 3 + 1] = sign * dD; part[h * 3 + 2] = sb; }
       }
     };
     for (int h = h0; h < h1; ++h) {
@@ -415,7 +427,7 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             xv[j] = in && (VEC || pq + j < pw) ? xv[j] : 0.f;
-            dv[j] = in && (VEC || pq + j < pw) ? dv[j] : 0.f;
+            dv[j] = in && (VEC || pq + j < pw) ? dv[j] * sign : 0.f;
             dd_part += xv[j] * dv[j];
           }
           if (gdz && t < here) {
@@ -563,7 +575,7 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
               for (int i = 0; i < 4; ++i) v[i] += pv[i];
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) out[i] = acc[k2][i] + Dh * v[i];
+            for (int i = 0; i < 4; ++i) out[i] = sign * (acc[k2][i] + Dh * v[i]);
             if (s < here) ssm_st4v<VEC>(gdx + s * ldo + hp + p, pw - p, out);
           }
         } else if (lane < 32) {
@@ -654,6 +666,8 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
 #pragma unroll
   for (int k = 0; k < CT; ++k) {
     const int t = 16 * (cg * CT + k) + c, n = 16 * nt + 4 * q;
+    accB[k] *= sign;
+    accC[k] *= sign;
     if (t < here) {
       const long o = (((long)b * f.T + t0 + t) * f.G + g) * f.N + n;
       const float vb[4] = {accB[k][0], accB[k][1], accB[k][2], accB[k][3]}, vc[4] = {accC[k][0], accC[k][1], accC[k][2], accC[k][3]};
