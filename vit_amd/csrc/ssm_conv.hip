@@ -2,6 +2,8 @@
 // backward and the single-token form:   u[t] = bias + sum_k w[k] x[t - K + 1 + k],  y = u or silu(u).
 // HBM bound: a thread owns V channels (one 16-byte access) of a strip of tokens and slides its window through registers, so
 // x is read once but for K - 1 tokens between strips (which the caches hold), and a wave reads 1 KB of a token's row.
+// At 8 x 2048 x 1792 bf16: forward 29 us (4.0 TB/s), backward 55 us (3.2 TB/s: u is recomputed, and windows and sums of 4 channels
+// leave four waves a SIMD), the parts' sum 4 us.
 #include "ssm_common.h"
 #include "rvit_internal.h"
 #include "ssm_args.h"

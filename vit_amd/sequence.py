@@ -179,7 +179,7 @@ class SSMStack(nn.Module):
         return x.unflatten(-1, (self.heads, self.HEAD)), Bm.unsqueeze(-2), Cm.unsqueeze(-2)
 
     def _start(self, x2d: torch.Tensor):
-        h = _Linear16.apply(x2d.to(BF16), self.weight_embed, self.bias_embed).float()
+        h = _Linear16.apply(x2d.to(BF16).contiguous(), self.weight_embed, self.bias_embed).float()
         return h, _Norm16.apply(h, self.pre_weight_l0, self.pre_bias_l0)
 
     def _join(self, k: int, h, y):
