@@ -324,39 +324,42 @@ __global__ __launch_bounds__(256, IT * V > 4 ? 2 : 4) void sandwich_bwd_kernel(S
   }
 }
 
-// columns of the parts, added in a fixed order: 16 threads take every 16th part of a column
+// columns of the parts, added in a fixed order: 16 threads take every 16th part of a column.  Rows 0 .. 3 of the grid: the
+// weights' and biases' sums; row 4 the channels' gates, or rows 4 and on, by turns, the samples' (over a sample's parts).
 __global__ __launch_bounds__(1024) void sandwich_sum_kernel(SandwichArgs a, int gate_bf16) {
   __shared__ double red[16][64];
   const int cx = threadIdx.x & 63, py = threadIdx.x >> 6;
-  const int k = blockIdx.y, e = blockIdx.x * 64 + cx;
-  double v = 0.0;
-  if (e < a.E) {
-    const long n = 5L * a.E, o = (long)k * a.E + e;
-    int p = py;
-    for (; p + 48 < a.parts; p += 64) {      // four loads on their way
-      const float u = a.part[p * n + o], w = a.part[(p + 16) * n + o], x = a.part[(p + 32) * n + o], y = a.part[(p + 48) * n + o];
-      v += ((double)u + (double)w) + ((double)x + (double)y);
+  const int e = blockIdx.x * 64 + cx;
+  const bool sample = blockIdx.y >= 4 && a.gate_kind == 2;
+  const int k = sample ? 4 : blockIdx.y;
+  const long n = 5L * a.E, samples = sample ? a.rows / a.T : 1;
+  const int parts = sample ? a.sample_parts : a.parts;
+  for (long b = sample ? blockIdx.y - 4 : 0; b < samples; b += gridDim.y - 4) {
+    const float* src = a.part + b * parts * n + (long)k * a.E + e;
+    double v = 0.0;
+    if (e < a.E) {
+      int p = py;
+      for (; p + 48 < parts; p += 64) {      // four loads on their way
+        const float u = src[p * n], w = src[(p + 16) * n], x = src[(p + 32) * n], y = src[(p + 48) * n];
+        v += ((double)u + (double)w) + ((double)x + (double)y);
+      }
+      for (; p < parts; p += 16) v += (double)src[p * n];
     }
-    for (; p < a.parts; p += 16) v += (double)a.part[p * n + o];
+    red[py][cx] = v;
+    __syncthreads();
+    if (py == 0 && e < a.E) {
+      for (int i = 1; i < 16; ++i) v += red[i][cx];
+      if (k == 4) {
+        if (gate_bf16) ((bf16*)a.dgate)[b * a.E + e] = (bf16)(float)v;
+        else ((float*)a.dgate)[b * a.E + e] = (float)v;
+      } else {
+        float* out = k == 0 ? a.dw1 : k == 1 ? a.db1 : k == 2 ? a.dw2 : a.db2;
+        if (out) out[e] = (float)v;
+      }
+    }
+    if (!sample) break;
+    __syncthreads();
   }
-  red[py][cx] = v;
-  __syncthreads();
-  if (py == 0 && e < a.E) {
-    for (int i = 1; i < 16; ++i) v += red[i][cx];
-    float* out = k == 0 ? a.dw1 : k == 1 ? a.db1 : k == 2 ? a.dw2 : k == 3 ? a.db2 : (float*)a.dgate;
-    if (k == 4 && gate_bf16) ((bf16*)out)[e] = (bf16)(float)v;
-    else if (out) out[e] = (float)v;
-  }
-}
-__global__ __launch_bounds__(256) void sandwich_sample_kernel(SandwichArgs a, int gate_bf16) {
-  const long n = a.rows / a.T * a.E, i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const long b = i / a.E;
-  const int e = i - b * a.E;
-  double v = 0.0;
-  for (int k = 0; k < a.sample_parts; ++k) v += (double)a.part[((b * a.sample_parts + k) * 5 + 4) * a.E + e];
-  if (gate_bf16) ((bf16*)a.dgate)[i] = (bf16)(float)v;
-  else ((float*)a.dgate)[i] = (float)v;
 }
 
 template <typename TR, typename TY, int V, int WPR, int IT>
@@ -364,13 +367,9 @@ int launch_bwd(const SandwichArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((sandwich_bwd_kernel<TR, TY, V, WPR, IT>), dim3(a.parts), dim3(256), 0, st, a);
   RVIT_CHECK_LAUNCH("sandwich_bwd");
   const int gb = a.gate_f32 ? 0 : (int)(sizeof(TY) == 2);
-  hipLaunchKernelGGL(sandwich_sum_kernel, dim3((a.E + 63) / 64, a.gate_kind == 1 ? 5 : 4), dim3(1024), 0, st, a, gb);
+  const long samples = a.gate_kind == 2 ? a.rows / a.T : a.gate_kind == 1;
+  hipLaunchKernelGGL(sandwich_sum_kernel, dim3((a.E + 63) / 64, (unsigned)(4 + (samples < 4096 ? samples : 4096))), dim3(1024), 0, st, a, gb);
   RVIT_CHECK_LAUNCH("sandwich_sum");
-  if (a.gate_kind == 2) {
-    const long n = a.rows / a.T * a.E;
-    hipLaunchKernelGGL(sandwich_sample_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a, gb);
-    RVIT_CHECK_LAUNCH("sandwich_sample");
-  }
   return RVIT_OK;
 }
 template <typename TR, typename TY, int V, int WPR, int IT>

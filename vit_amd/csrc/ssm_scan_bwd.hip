@@ -189,7 +189,7 @@ __global__ __launch_bounds__(256, 2) void ssm_scan_bwd_state_kernel(SsmBwdArgs a
 // before it is worked on, its states while its scores are.
 // [8, 2048, 24, 64] x 128 states, bf16: 285 - 295 us for 0.7 GB (2.5 TB/s).  Its LDS and registers allow one workgroup, two waves a
 // SIMD: vector instructions (three-part operands, decays, sums) are a quarter of a wave's time, so half of the SIMD's, matrix
-// instructions a twelfth, LDS is busy for 40 %; the rest waits at the head's four barriers.  64 windows of 8 tokens, fp32: 30 us.
+// instructions a twelfth, LDS is busy for 40 %; the rest waits, at the head's three barriers and for LDS.  64 windows of 8 tokens, fp32: 30 us.
 template <typename T, int NP>
 struct BwdLds {
   using O = SsmOps<T>;
@@ -687,23 +687,24 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
   }
 }
 
-// dB, dC: the parts of a group's heads, added in their order
+// The sums behind the chunks, in a fixed order, in one launch.  The first H workgroups: dA, dD, ddt_bias of a head from its chunks'
+// parts, in 64 bits; the others (n > 1): dB, dC from the n parts of a group's heads.
 template <typename T>
-__global__ __launch_bounds__(256) void ssm_dbc_sum_kernel(const float* part, T* dB, T* dC, long whole, int n) {
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < 2 * whole; i += (long)gridDim.x * 256) {
-    float v = 0.f;
-    for (int k = 0; k < n; ++k) v += part[(long)k * 2 * whole + i];
-    if (i < whole) ssm_st(dB + i, v);
-    else ssm_st(dC + i - whole, v);
-  }
-}
-
-// dA, dD, ddt_bias: one workgroup per head over the chunks' parts, summed in 64 bits in a fixed order
-__global__ __launch_bounds__(256) void ssm_head_sum_kernel(const float* part, float* dA, float* dD, float* db, long n, int H) {
+__global__ __launch_bounds__(256) void ssm_bwd_sum_kernel(const float* part, float* dA, float* dD, float* db, long chunks, int H, const float* dbc, T* dB, T* dC,
+                                                          long whole, int n) {
   __shared__ double red[4][3];
+  if ((int)blockIdx.x >= H) {
+    for (long i = (long)(blockIdx.x - H) * 256 + threadIdx.x; i < 2 * whole; i += (long)(gridDim.x - H) * 256) {
+      float v = 0.f;
+      for (int k = 0; k < n; ++k) v += dbc[(long)k * 2 * whole + i];
+      if (i < whole) ssm_st(dB + i, v);
+      else ssm_st(dC + i - whole, v);
+    }
+    return;
+  }
   const int h = blockIdx.x;
   double v[3] = {0.0, 0.0, 0.0};
-  for (long i = threadIdx.x; i < n; i += 256)
+  for (long i = threadIdx.x; i < chunks; i += 256)
 #pragma unroll
     for (int k = 0; k < 3; ++k) v[k] += (double)part[(i * H + h) * 3 + k];
 #pragma unroll
@@ -740,15 +741,10 @@ int launch_bwd(const SsmBwdArgs& a, hipStream_t st) {
   }
   hipLaunchKernelGGL((ssm_scan_bwd_chunk_kernel<T, NP, VEC>), dim3((unsigned)((long)f.B * f.nchunks * f.G * a.hsplit)), dim3(512), cb, st, a);
   RVIT_CHECK_LAUNCH("ssm_scan_bwd_chunk");
-  const long whole = (long)f.B * f.T * f.G * f.N;
-  if (a.hsplit > 1) {
-    const long blocks = (2 * whole + 255) / 256;
-    hipLaunchKernelGGL((ssm_dbc_sum_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, a.dbc_part, (T*)a.dB, (T*)a.dC,
-                       whole, a.hsplit);
-    RVIT_CHECK_LAUNCH("ssm_dbc_sum");
-  }
-  hipLaunchKernelGGL(ssm_head_sum_kernel, dim3(f.H), dim3(256), 0, st, a.part, a.dA, a.dD, a.dbias, (long)f.B * f.nchunks, f.H);
-  RVIT_CHECK_LAUNCH("ssm_head_sum");
+  const long whole = (long)f.B * f.T * f.G * f.N, blocks = a.hsplit > 1 ? (2 * whole + 255) / 256 : 0;
+  hipLaunchKernelGGL((ssm_bwd_sum_kernel<T>), dim3((unsigned)(f.H + (blocks < 4096 ? blocks : 4096))), dim3(256), 0, st, a.part, a.dA, a.dD, a.dbias,
+                     (long)f.B * f.nchunks, f.H, a.dbc_part, (T*)a.dB, (T*)a.dC, whole, a.hsplit);
+  RVIT_CHECK_LAUNCH("ssm_bwd_sum");
   return RVIT_OK;
 }
 
