@@ -536,3 +536,58 @@ def test_mixed_devices_are_refused(dev):
         ssm.causal_conv(torch.zeros(1, 4, 4, device=dev), torch.zeros(4, 4))
     with pytest.raises(ValueError, match="cpu"):
         ssm.sandwich_norm(torch.zeros(3, 8, device=dev), torch.zeros(3, 8), torch.ones(8, device=dev), None, torch.ones(8, device=dev), None)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_scan_lengths_over_segments(dev, dtype):
+    """A sequence that is cut into segments, with samples that end before, inside and at the borders of them."""
+    from vit_amd import ssm
+    T = 640
+    lens = torch.tensor([0, 70, 256, 257, 640, 639], dtype=torch.int32)
+    s = scan_inputs(80, DTYPES[dtype], len(lens), T, 2, 24, 1, 20, state=True)
+    want_in = leaves64(s)
+    wy, wend = ref.selective_scan(**want_in, lengths=lens)
+    g = torch.Generator().manual_seed(81)
+    dy, dend = randn(g, *wy.shape, dtype=DTYPES[dtype]), randn(g, *wend.shape)
+    want = torch.autograd.grad([wy, wend], [want_in[k] for k in SCAN_NAMES], [dy.double(), dend.double()])
+    behind = torch.arange(T)[None] >= lens[:, None]
+    for k in ("x", "dt", "Bm", "Cm", "z"):
+        s[k][behind] = float("nan")
+    dy[behind] = float("nan")
+    d = {k: v.requires_grad_() for k, v in to(s, dev).items()}
+    y, end = _call(ssm, d, lengths=lens.to(dev), return_state=True)
+    close("y", y, wy)
+    close("end", end, wend)
+    for k, a, b in zip(SCAN_NAMES, torch.autograd.grad([y, end], [d[k] for k in SCAN_NAMES], [dy.to(dev), dend.to(dev)]), want):
+        close("d" + k, a, b)
+
+
+def test_kept_states_past_32_bits(dev):
+    """4300 chunks of 64 heads x 64 x 128 states: more than 2^31 kept values, inputs past 2^31 bytes.  The end of the sequence against
+    the same tokens alone on the state that the first part leaves."""
+    from vit_amd import ssm
+    T, T0, H, P, N = 4300 * 64 - 7, 4290 * 64, 64, 64, 128
+    g = torch.Generator(device=dev).manual_seed(90)
+    r = lambda *shape: torch.randn(*shape, generator=g, device=dev, dtype=torch.bfloat16)  # noqa: E731
+    s = dict(x=r(1, T, H, P), dt=r(1, T, H), Bm=r(1, T, 1, N), Cm=r(1, T, 1, N), z=r(1, T, H, P), A=-torch.rand(H, generator=g, device=dev) - 0.5,
+             D=torch.rand(H, generator=g, device=dev), dt_bias=torch.full((H,), -3.0, device=dev), state=None)
+    over = ("x", "dt", "Bm", "Cm", "z")
+    leaf = {k: v.requires_grad_() if k in over else v for k, v in s.items()}
+    dy = torch.zeros(1, T, H, P, device=dev, dtype=torch.bfloat16)
+    dy[:, T0:] = r(1, T - T0, H, P)
+    y = _call(ssm, leaf)
+    grads = [v[:, T0:].clone() for v in torch.autograd.grad(y, [leaf[k] for k in over], dy)]
+    y = y.detach()[:, T0:].clone()
+    with torch.no_grad():
+        _, state = _call(ssm, {k: v[:, :T0] if k in over else v for k, v in s.items()}, return_state=True)
+    tail = {k: v.detach()[:, T0:].clone().requires_grad_() if k in over else v for k, v in s.items()}
+    tail["state"] = state
+    yt = _call(ssm, tail)
+    # (two runs of the same definition: each within the tolerance of it)
+    err = float((y.double() - yt.detach().double()).norm() / yt.detach().double().norm())
+    assert err <= 2 * (2.0 ** -8 + 2.0 ** -10), err
+    for k, a, b in zip(over, grads, torch.autograd.grad(yt, [tail[k] for k in over], dy[:, T0:])):
+        err = float((a.double() - b.double()).norm() / b.double().norm())
+        assert err <= 2 * (2.0 ** -8 + 2.0 ** -10), (k, err)
+    del leaf, s, tail, grads, y, yt, dy, state
+    torch.cuda.empty_cache()

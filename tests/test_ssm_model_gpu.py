@@ -135,3 +135,14 @@ def test_checkpoint_round_trip(dev, tmp_path):
     sc = StreamingClassifier(path, carry_state=True)
     f = torch.randn(1, 128, device=dev)
     assert torch.equal(sc.model.forward_temporal_step(f)[0], m.forward_temporal_step(f)[0])
+
+
+def test_a_frame_out_of_a_window_of_bf16_features(dev):
+    """Features that already are bf16 come as a slice of a longer window: rows apart in memory."""
+    m = _model(dev).eval()
+    f = torch.randn(3, 4, 128, device=dev).bfloat16()
+    with torch.no_grad():
+        a, b = m.forward_temporal_step(f[:, 1])[0], m.forward_temporal_step(f[:, 1].contiguous())[0]
+        assert torch.equal(a, b)
+        x = torch.randn(4, 3, 128, device=dev).bfloat16().transpose(0, 1)
+        assert torch.equal(m.forward_temporal_only(x), m.forward_temporal_only(x.contiguous()))
