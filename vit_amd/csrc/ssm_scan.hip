@@ -137,7 +137,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_
   if (YOUT && a.nseg > 1) get_state(a.seg_state + seg * a.seg_stride, true);     // written by the join
   else if (YOUT && a.state0) get_state(a.state0, false);
   double total = 0.0;
-  // wave 0: the decays of a chunk from its dt (one token a lane)
+  // the wave with the fewest scores: the decays of a chunk from its dt (one token a lane)
   auto fetch_dt = [&](int ch) { return dt[(long)min(ch * Q + lane, len - 1) * a.sdt]; };
   auto decay = [&](T raw, int ch) {
     float* sd = decays + (ch & 1) * 5 * Q;
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_
   T raw = (T)0.f;
   if (c0 < cl) {
     fetch(c0);
-    if (w == 0) {
+    if (tw == 0) {
       decay(fetch_dt(c0), c0);
       raw = fetch_dt(c0 + 1);
     }
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_
     const bool more = ch + 1 < cl;
     if (more) fetch(ch + 1);
     if (YOUT && a.states) put_state(a.states + (long)ch * a.seg_stride, true);
-    if (w == 0 && more) {
+    if (tw == 0 && more) {
       decay(raw, ch + 1);
       raw = fetch_dt(ch + 2);
     }
@@ -292,7 +292,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_
     if (a.state_out && seg == a.nseg - 1) put_state(a.state_out, false);
   } else {
     put_state(a.seg_state + seg * a.seg_stride, true);
-    if (threadIdx.x == 0 && pb == 0) a.seg_decay[((long)seg * a.B + b) * a.H + h] = total;
+    if (tw == 0 && lane == 0 && pb == 0) a.seg_decay[((long)seg * a.B + b) * a.H + h] = total;
   }
 }
 
