@@ -69,11 +69,12 @@ __device__ __forceinline__ void scores(const T* Bs, const T* Cs, T* Gs, const fl
 // A chunk's images and decays are fetched and worked out while the chunk before it is computed.
 // YOUT = false: only the state a segment (but the last) reaches from zero, and the segment's summed log decay (long sequences of few
 // rows are cut into segments, joined by ssm_join_kernel).  VEC: all wide accesses are aligned and whole.
-// Measured, bf16, 128 states: 32768 tokens x 16 heads x 64 (segments of 16 chunks) 119 us, the pass for states 45 us;
-// [8, 2048, 24, 64] with a state kept per chunk (0.4 GB) 160 us and 39 us.  Bound by two waves a SIMD (256 registers, 69 KB of LDS):
+// Measured, bf16, 128 states: 32768 tokens x 16 heads x 64 (segments of 16 chunks) 112 us, the pass for states 44 us;
+// [8, 2048, 24, 64] with a state kept per chunk (0.4 GB) 157 us and 39 us.  Bound by two waves a SIMD (256 registers, 69 KB of LDS):
 // vector instructions (splits, decays, the gate) fill a fifth to a quarter of a wave's time, matrix instructions a tenth, waits for
 // LDS, barriers and memory the rest.  A second x image with two barriers a chunk, and one barrier in the pass for states,
-// took the same time.
+// took the same time, as did the score tiles spread evenly over the waves; the decays are worked out by the wave with the fewest of
+// them (by wave 0 of every workgroup: 120 and 161 us).
 template <typename T, int NP, bool YOUT, bool VEC>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_scan_fwd_kernel(SsmScanArgs a) {
   using O = SsmOps<T>;
