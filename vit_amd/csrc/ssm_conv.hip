@@ -2,8 +2,8 @@
 // backward and the single-token form:   u[t] = bias + sum_k w[k] x[t - K + 1 + k],  y = u or silu(u).
 // HBM bound: a thread owns V channels (one 16-byte access) of a strip of tokens and slides its window through registers, so
 // x is read once but for K - 1 tokens between strips (which the caches hold), and a wave reads 1 KB of a token's row.
-// At 8 x 2048 x 1792 bf16: forward 29 us (4.0 TB/s), backward 55 us (3.2 TB/s: u is recomputed, and windows and sums of 4 channels
-// leave four waves a SIMD), the parts' sum 4 us.
+// At 8 x 2048 x 1792 bf16: forward 29 us (4.0 TB/s), backward 52 us (3.4 TB/s: u is recomputed, and windows and sums of 4 channels
+// leave four waves a SIMD; more tokens on their way change nothing), the parts' sum 4 us.
 #include "ssm_common.h"
 #include "rvit_internal.h"
 #include "ssm_args.h"
@@ -132,9 +132,9 @@ __global__ __launch_bounds__(256) void ssm_conv_fwd_kernel(SsmConvArgs a) {
 
 // du[t] = dy silu'(u), u recomputed; dx[t] = sum_k w[k] du[t + K - 1 - k]; dw[k] = sum_t du[t] x[t - K + 1 + k]; db = sum du.
 // A workgroup is 32 channel groups wide and 8 strips deep; its strips' dw, db are added in LDS in a fixed order and
-// written as one part, which ssm_conv_sum_kernel adds.
+// written as one part, which ssm_conv_sum_kernel adds.  (Three waves a SIMD for windows of 5 and 6: four would spill.)
 template <typename T, int V, int K>
-__global__ __launch_bounds__(256, 4) void ssm_conv_bwd_kernel(SsmConvArgs a) {
+__global__ __launch_bounds__(256, V >= 4 && K >= 5 ? 3 : 4) void ssm_conv_bwd_kernel(SsmConvArgs a) {
   __shared__ float red[8][32][V];
   const int groups = a.C / V;
   const int gx = threadIdx.x & 31, sy = threadIdx.x >> 5;
@@ -167,54 +167,56 @@ __global__ __launch_bounds__(256, 4) void ssm_conv_bwd_kernel(SsmConvArgs a) {
       nx.load(x + min(t0, len - 1) * a.sxt);
       ny.load(dy + min(t0, len - 1) * a.syt);
     }
-    for (int t = t0; t < t1 + K - 1; ++t) {
-      float g[V];
-      zero<V>(win[K - 1]);
-      zero<V>(g);
-      if (t < len) {
-        nx.get(win[K - 1]);
-        ny.get(g);
-        nx.load(x + min(t + 1, len - 1) * a.sxt);
-        ny.load(dy + min(t + 1, len - 1) * a.syt);
-      }
+    // (K tokens a turn, the windows' places in turn: nothing moves)
+    for (int tk = t0; tk < t1 + K - 1; tk += K) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (a.silu) {
-          float u = bias[j];
-#pragma unroll
-          for (int k = 0; k < K; ++k) u = fmaf(w[k][j], win[k][j], u);
-          const float sg = ssm_sigmoid(u);
-          g[j] = t < len ? g[j] * (sg + u * sg * (1.f - sg)) : 0.f;
+      for (int ph = 0; ph < K; ++ph) {
+        const int t = tk + ph;
+        if (t >= t1 + K - 1) break;
+        auto at = [&](int k) { return (k + ph) % K; };      // place of token t - (K - 1) + k
+        float g[V];
+        zero<V>(win[at(K - 1)]);
+        zero<V>(g);
+        if (t < len) {
+          nx.get(win[at(K - 1)]);
+          ny.get(g);
+          nx.load(x + min(t + 1, len - 1) * a.sxt);
+          ny.load(dy + min(t + 1, len - 1) * a.syt);
         }
-        du[K - 1][j] = g[j];
-        const float own = t < t1 ? g[j] : 0.f;      // (the tokens behind the strip are another's)
-        db[j] += own;
 #pragma unroll
-        for (int k = 0; k < K; ++k) dw[k][j] = fmaf(own, win[k][j], dw[k][j]);
-      }
-      const int to = t - (K - 1);
-      float o[V];
+        for (int j = 0; j < V; ++j) {
+          if (a.silu) {
+            float u = bias[j];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        o[j] = 0.f;
+            for (int k = 0; k < K; ++k) u = fmaf(w[k][j], win[at(k)][j], u);
+            const float sg = ssm_sigmoid(u);
+            g[j] = t < len ? g[j] * (sg + u * sg * (1.f - sg)) : 0.f;
+          }
+          du[at(K - 1)][j] = g[j];
+          const float own = t < t1 ? g[j] : 0.f;      // (the tokens behind the strip are another's)
+          db[j] += own;
 #pragma unroll
-        for (int k = 0; k < K; ++k) o[j] = fmaf(w[k][j], du[K - 1 - k][j], o[j]);
-      }
-      // du[i] holds token t - (K - 1) + i, so o is dx of token `to`: complete for to >= t0, and for the kept inputs
-      if (to >= t0 || s == 0) {
-        if (dso && to >= len - (K - 1) && to < len) {
-          float v[V];
-          ldv<T, V>(dso + (long)(to - len + K - 1) * a.C, v);
-#pragma unroll
-          for (int j = 0; j < V; ++j) o[j] += v[j];
+          for (int k = 0; k < K; ++k) dw[k][j] = fmaf(own, win[at(k)][j], dw[k][j]);
         }
-        if (to >= 0) stv<T, V>(dx + (long)to * a.C, o);
-        else if (a.dstate) stv<T, V>((T*)a.dstate + ((long)b * (K - 1) + to + K - 1) * a.C + c0, o);
-      }
+        const int to = t - (K - 1);
+        float o[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
+        for (int j = 0; j < V; ++j) {
+          o[j] = 0.f;
 #pragma unroll
-        for (int k = 0; k + 1 < K; ++k) { win[k][j] = win[k + 1][j]; du[k][j] = du[k + 1][j]; }
+          for (int k = 0; k < K; ++k) o[j] = fmaf(w[k][j], du[at(K - 1 - k)][j], o[j]);
+        }
+        // du's place at(i) holds token t - (K - 1) + i, so o is dx of token `to`: complete for to >= t0, and for the kept inputs
+        if (to >= t0 || s == 0) {
+          if (dso && to >= len - (K - 1) && to < len) {
+            float v[V];
+            ldv<T, V>(dso + (long)(to - len + K - 1) * a.C, v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) o[j] += v[j];
+          }
+          if (to >= 0) stv<T, V>(dx + (long)to * a.C, o);
+          else if (a.dstate) stv<T, V>((T*)a.dstate + ((long)b * (K - 1) + to + K - 1) * a.C + c0, o);
+        }
       }
     }
   }
@@ -290,13 +292,15 @@ __global__ __launch_bounds__(256) void ssm_conv_step_kernel(SsmConvArgs a) {
 template <typename T, int V, int K>
 int launch(const SsmConvArgs& a, int what, hipStream_t st) {
   const int groups = a.C / V;
-  if (what == SSM_CONV_BWD) {
-    const int sblocks = (a.strips + 7) / 8;
-    hipLaunchKernelGGL((ssm_conv_bwd_kernel<T, V, K>), dim3((unsigned)((groups + 31) / 32) * (a.B * sblocks)), dim3(256), 0, st, a);
-    RVIT_CHECK_LAUNCH("ssm_conv_bwd");
-    hipLaunchKernelGGL(ssm_conv_sum_kernel, dim3((unsigned)(((long)(K + 1) * a.C + 63) / 64)), dim3(1024), 0, st, a.part, a.dw, a.dbias, a.B * sblocks, a.C, K);
-    RVIT_CHECK_LAUNCH("ssm_conv_sum");
-    return RVIT_OK;
+  if constexpr (V < 8) {      // (eight channels a thread: forward only, see below)
+    if (what == SSM_CONV_BWD) {
+      const int sblocks = (a.strips + 7) / 8;
+      hipLaunchKernelGGL((ssm_conv_bwd_kernel<T, V, K>), dim3((unsigned)((groups + 31) / 32) * (a.B * sblocks)), dim3(256), 0, st, a);
+      RVIT_CHECK_LAUNCH("ssm_conv_bwd");
+      hipLaunchKernelGGL(ssm_conv_sum_kernel, dim3((unsigned)(((long)(K + 1) * a.C + 63) / 64)), dim3(1024), 0, st, a.part, a.dw, a.dbias, a.B * sblocks, a.C, K);
+      RVIT_CHECK_LAUNCH("ssm_conv_sum");
+      return RVIT_OK;
+    }
   }
   const long n = (long)a.B * (what == SSM_CONV_FWD ? a.strips : 1) * groups;
   const dim3 grid((unsigned)((n + 255) / 256));
@@ -319,7 +323,7 @@ int launch_k(const SsmConvArgs& a, int what, hipStream_t st) {
 }  // namespace
 
 int rvit_ssm_conv_impl(const SsmConvArgs& a, int dtype, int what, hipStream_t st) {
-  // (bf16 backward: four channels a thread; with eight its windows and sums leave three waves a SIMD: 77 us against 52 at 8 x 2048 x 1792)
+  // (bf16 backward: four channels a thread; with eight its windows and sums leave three waves a SIMD: 77 us against 55 at 8 x 2048 x 1792)
   if (dtype == RVIT_BF16) {
     if (!a.vec) return launch_k<bf16, 1>(a, what, st);
     return what == SSM_CONV_BWD ? launch_k<bf16, 4>(a, what, st) : launch_k<bf16, 8>(a, what, st);
