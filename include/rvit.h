@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define RVIT_ABI_VERSION 30
+#define RVIT_ABI_VERSION 31
 
 #define RVIT_BF16 0
 #define RVIT_F32 1
@@ -661,7 +661,7 @@ int rvit_ssm_conv_step(const void* x, int64_t sxb, const float* w, const float* 
  * x, z, y [B,T,H,P]; dt [B,T,H]; Bm, Cm [B,T,G,N] (shared by the H / G heads of a group), one dtype; A, D, dt_bias fp32 [H];
  * states fp32 [B,H,P,N], 1 <= N <= 128.  Inputs have strides per sample and token in elements ([H,P], [G,N], [H] packed);
  * outputs are packed.  D, z, dt_bias, state0, lengths, state_out may be null.  lengths as above: the returned state is the one
- * behind the last token of each sample.  Training passes v (dtype, [B,T,H,P]; only with z) and states (fp32, state_floats of
+ * behind the last token of each sample.  Training passes v (fp32, [B,T,H,P]; only with z) and states (fp32, state_floats of
  * rvit_ssm_scan_plan), both read by bwd.  Workspaces: fwd_bytes / bwd_bytes of rvit_ssm_scan_plan, 16-byte aligned.  bwd:
  * dA, dD, ddt_bias fp32 [H] (the last two may be null), dstate0 may be null, dz with z only.  Results do not depend on the
  * order in which workgroups run.  A non-finite input of a valid token may reach every output of its chunk of 64 tokens.
@@ -671,11 +671,11 @@ int rvit_ssm_scan_plan(int64_t* fwd_bytes, int64_t* state_floats, int64_t* bwd_b
 int rvit_ssm_scan_fwd(const void* x, int64_t sxb, int64_t sxt, const void* dt, int64_t sdb, int64_t sdt, const float* A,
                       const void* Bm, int64_t sbb, int64_t sbt, const void* Cm, int64_t scb, int64_t sct, const float* D,
                       const void* z, int64_t szb, int64_t szt, const float* dt_bias, const float* state0, const int* lengths,
-                      void* y, void* v, float* state_out, float* states, void* workspace, int64_t workspace_bytes, int dtype,
+                      void* y, float* v, float* state_out, float* states, void* workspace, int64_t workspace_bytes, int dtype,
                       int B, int T, int H, int P, int G, int N, void* stream);
 int rvit_ssm_scan_bwd(const void* x, int64_t sxb, int64_t sxt, const void* dt, int64_t sdb, int64_t sdt, const float* A,
                       const void* Bm, int64_t sbb, int64_t sbt, const void* Cm, int64_t scb, int64_t sct, const float* D,
-                      const void* z, int64_t szb, int64_t szt, const float* dt_bias, const int* lengths, const void* v,
+                      const void* z, int64_t szb, int64_t szt, const float* dt_bias, const int* lengths, const float* v,
                       const float* states, const void* dy, int64_t syb, int64_t syt, const float* dstate_out, void* dx,
                       void* ddt, float* dA, void* dB, void* dC, float* dD, void* dz, float* ddt_bias, float* dstate0,
                       void* workspace, int64_t workspace_bytes, int dtype, int B, int T, int H, int P, int G, int N,

@@ -91,7 +91,7 @@ int rvit_ssm_scan_plan(int64_t* fwd_bytes, int64_t* state_floats, int64_t* bwd_b
 
 int rvit_ssm_scan_fwd(const void* x, int64_t sxb, int64_t sxt, const void* dt, int64_t sdb, int64_t sdt, const float* A, const void* Bm,
                       int64_t sbb, int64_t sbt, const void* Cm, int64_t scb, int64_t sct, const float* D, const void* z, int64_t szb, int64_t szt,
-                      const float* dt_bias, const float* state0, const int* lengths, void* y, void* v, float* state_out, float* states,
+                      const float* dt_bias, const float* state0, const int* lengths, void* y, float* v, float* state_out, float* states,
                       void* workspace, int64_t workspace_bytes, int dtype, int B, int T, int H, int P, int G, int N, void* stream) {
   SsmScanArgs a = {};
   if (int e = shape(a, dtype, B, T, H, P, G, N)) return e;
@@ -101,7 +101,7 @@ int rvit_ssm_scan_fwd(const void* x, int64_t sxb, int64_t sxt, const void* dt, i
   RVIT_CHECK_ARG(seg_bytes(a) == 0 || (workspace && workspace_bytes >= seg_bytes(a) + 16), "ssm_scan_fwd: workspace of %lld bytes, %lld needed",
                  (long long)workspace_bytes, (long long)seg_bytes(a) + 16);
   a.state0 = state0; a.y = y; a.v = v; a.state_out = state_out; a.states = states;
-  a.vec_y = at(y, 4 * es(dtype)) && at(v, 4 * es(dtype)) && P % 4 == 0;
+  a.vec_y = at(y, 4 * es(dtype)) && at(v, 16) && P % 4 == 0;
   a.vec_state = N % 4 == 0 && at(state0, 16) && at(state_out, 16);
   RVIT_CHECK_ARG(at(states, 16), "ssm_scan_fwd: states alignment");
   char* ws = (char*)workspace;
@@ -111,7 +111,7 @@ int rvit_ssm_scan_fwd(const void* x, int64_t sxb, int64_t sxt, const void* dt, i
 
 int rvit_ssm_scan_bwd(const void* x, int64_t sxb, int64_t sxt, const void* dt, int64_t sdb, int64_t sdt, const float* A, const void* Bm,
                       int64_t sbb, int64_t sbt, const void* Cm, int64_t scb, int64_t sct, const float* D, const void* z, int64_t szb, int64_t szt,
-                      const float* dt_bias, const int* lengths, const void* v, const float* states, const void* dy, int64_t syb, int64_t syt,
+                      const float* dt_bias, const int* lengths, const float* v, const float* states, const void* dy, int64_t syb, int64_t syt,
                       const float* dstate_out, void* dx, void* ddt, float* dA, void* dB, void* dC, float* dD, void* dz, float* ddt_bias,
                       float* dstate0, void* workspace, int64_t workspace_bytes, int dtype, int B, int T, int H, int P, int G, int N, void* stream) {
   SsmBwdArgs a = {};
@@ -124,10 +124,10 @@ int rvit_ssm_scan_bwd(const void* x, int64_t sxb, int64_t sxt, const void* dt, i
   if (int e = rvit_ssm_scan_plan(nullptr, nullptr, &need, B, T, H, P, G, N)) return e;
   RVIT_CHECK_ARG(workspace && at(workspace, 16) && workspace_bytes >= need, "ssm_scan_bwd: workspace of %lld bytes, %lld needed",
                  (long long)workspace_bytes, (long long)need);
-  a.f.v = (void*)v; a.f.states = (float*)states;
+  a.f.v = (float*)v; a.f.states = (float*)states;
   a.dy = dy; a.syb = syb; a.syt = syt; a.dstate_out = dstate_out;
   a.dx = dx; a.dz = z ? dz : nullptr; a.ddt = ddt; a.dB = dB; a.dC = dC; a.dA = dA; a.dD = dD; a.dbias = ddt_bias; a.dstate0 = dstate0;
-  a.f.vec_y = at(v, 4 * es(dtype)) && P % 4 == 0;
+  a.f.vec_y = at(v, 16) && P % 4 == 0;
   a.f.vec_state = N % 4 == 0 && at(dstate_out, 16) && at(dstate0, 16);
   RVIT_CHECK_ARG(at(states, 16), "ssm_scan_bwd: states alignment");
   a.vec_dy = at(dy, 4 * es(dtype)) && syt < MOST && syb % 4 == 0 && syt % 4 == 0 && P % 4 == 0;

@@ -11,7 +11,8 @@ struct SsmScanArgs {
   const float *A, *D, *dt_bias, *state0;
   const int* lengths;
   void* y;
-  void* v;               // v before the gate, kept for the backward pass (or null)
+  float* v;              // v before the gate, kept for the backward pass (or null): in 32 bits, as dz = dy v silu'(z) of bf16 calls would
+                         // else be rounded twice
   float* state_out;      // [B,H,P,N] or null
   // Inner copies of states are padded to pblocks * 64 channels x NP states (NP: N up to 32, 64 or 128; what is added is zero) and
   // lie as [B, H, pblocks, NP / 4, 64, 4], so that a wave's piece of its 16 x 16 tiles is four runs of 256 bytes.  (With rows

@@ -105,7 +105,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_
   const T* dt = (const T*)a.dt + b * a.sdb + h;
   const T* z = a.z ? (const T*)a.z + b * a.szb + (long)h * a.P + pb * 64 : nullptr;
   T* y = YOUT ? (T*)a.y + ((long)b * a.T * a.H + h) * a.P + pb * 64 : nullptr;
-  T* v_out = YOUT && a.v ? (T*)a.v + ((long)b * a.T * a.H + h) * a.P + pb * 64 : nullptr;
+  float* v_out = YOUT && a.v ? a.v + ((long)b * a.T * a.H + h) * a.P + pb * 64 : nullptr;
   const long ldy = (long)a.H * a.P;
   const double A2 = (double)a.A[h] * 1.4426950408889634;   // log2 e: decays in base-2 units
   const float bias = a.dt_bias ? a.dt_bias[h] : 0.f;
@@ -288,7 +288,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_
     const int from = max(c0, cl) * Q, to = min(c1 * Q, a.T);
     for (long i = threadIdx.x; i < (long)(to - from) * 64; i += 256) {
       const int t = from + (int)(i >> 6), p = (int)(i & 63);
-      if (p < pw) { ssm_st(y + t * ldy + p, 0.f); if (v_out) ssm_st(v_out + t * ldy + p, 0.f); }
+      if (p < pw) { ssm_st(y + t * ldy + p, 0.f); if (v_out) v_out[t * ldy + p] = 0.f; }
     }
     if (a.state_out && seg == a.nseg - 1) put_state(a.state_out, false);
   } else {

@@ -270,13 +270,14 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
     const T* gx = (const T*)f.x + b * f.sxb + t0 * f.sxt;
     const T* gdy = (const T*)a.dy + b * a.syb + t0 * a.syt;
     const T* gz = f.z ? (const T*)f.z + b * f.szb + t0 * f.szt : nullptr;
-    const T* gv = f.z ? (const T*)f.v + ((long)b * f.T + t0) * ldo : nullptr;
+    const float* gv = f.z ? f.v + ((long)b * f.T + t0) * ldo : nullptr;
     const T* gdt = (const T*)f.dt + b * f.sdb + (long)(t0 + min(lane, live - 1)) * f.sdt;
     T* gdx = (T*)a.dx + ((long)b * f.T + t0) * ldo;
     T* gdz = a.dz ? (T*)a.dz + ((long)b * f.T + t0) * ldo : nullptr;
     // a head's x, dy, z, v: two pieces of four channels a thread, token row and row + 32
     const int row = threadIdx.x >> 4, pq = (threadIdx.x & 15) * 4;
-    SsmRaw4<T> xr[2], dr[2], zr[2], vr[2];
+    SsmRaw4<T> xr[2], dr[2], zr[2];
+    SsmRaw4<float> vr[2];
     f32x4 dsn[NP / 32];
     T rawn = (T)0.f;
     float* Ds = (float*)(smem + L::DS);
@@ -299,7 +300,7 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
         if (VEC) {
           // token strides are under 2^24 here: 32-bit offsets from a uniform address
           const unsigned p = pq < pw ? pq : 0;
-          auto at = [&](const T* base, long st) { return (const T*)((const char*)(base + hp) + ((unsigned)t * (unsigned)st + p) * (unsigned)sizeof(T)); };
+          auto at = [&](auto* base, long st) { return (decltype(base))((const char*)(base + hp) + ((unsigned)t * (unsigned)st + p) * (unsigned)sizeof(*base)); };
           xr[i].load(at(gx, f.sxt));
           dr[i].load(at(gdy, a.syt));
           if (gz) {

@@ -206,12 +206,12 @@ ScanOut scan_run(const Tensor& x, const Tensor& dt, const Tensor& A, const Tenso
   ScanOut o;
   o.y = like(x);
   if (want_state) o.after = at::empty({d.B, d.H, d.P, d.N}, A.options());
-  if (train && z.defined()) o.v = like(x);
+  if (train && z.defined()) o.v = at::empty(x.sizes(), A.options());
   if (train) o.states = at::empty({floats}, A.options());
   const Tensor ws = fwd > 16 ? bytes(fwd, x) : Tensor();
   done(rvit_ssm_scan_fwd(ptr(x), x.stride(0), x.stride(1), ptr(dt), dt.stride(0), dt.stride(1), A.data_ptr<float>(), ptr(Bm), Bm.stride(0), Bm.stride(1), ptr(Cm),
                          Cm.stride(0), Cm.stride(1), (const float*)ptr(D), ptr(z), stride(z, 0), stride(z, 1), (const float*)ptr(dt_bias), (const float*)ptr(state),
-                         (const int*)ptr(lengths), ptr(o.y), ptr(o.v), (float*)ptr(o.after), (float*)ptr(o.states), ptr(ws), fwd, dtype(x), d.B, d.T, d.H, d.P, d.G,
+                         (const int*)ptr(lengths), ptr(o.y), (float*)ptr(o.v), (float*)ptr(o.after), (float*)ptr(o.states), ptr(ws), fwd, dtype(x), d.B, d.T, d.H, d.P, d.G,
                          d.N, stream(x)),
        "rvit_ssm_scan_fwd");
   return o;
@@ -249,7 +249,7 @@ struct Scan : torch::autograd::Function<Scan> {
       const Tensor ws = bytes(nb, x);
       done(rvit_ssm_scan_bwd(ptr(x), x.stride(0), x.stride(1), ptr(dt), dt.stride(0), dt.stride(1), A.data_ptr<float>(), ptr(Bm), Bm.stride(0), Bm.stride(1), ptr(Cm),
                              Cm.stride(0), Cm.stride(1), (const float*)ptr(D), ptr(z), stride(z, 0), stride(z, 1), (const float*)ptr(dt_bias),
-                             (const int*)ptr(lengths), ptr(v), (const float*)ptr(states), ptr(dy), dy.stride(0), dy.stride(1), (const float*)ptr(dafter), ptr(dx),
+                             (const int*)ptr(lengths), (const float*)ptr(v), (const float*)ptr(states), ptr(dy), dy.stride(0), dy.stride(1), (const float*)ptr(dafter), ptr(dx),
                              ptr(ddt), dA.data_ptr<float>(), ptr(dB), ptr(dC), (float*)ptr(dD), ptr(dz), (float*)ptr(dbias), (float*)ptr(ds), ptr(ws), nb, dtype(x),
                              d.B, d.T, d.H, d.P, d.G, d.N, stream(x)),
            "rvit_ssm_scan_bwd");
