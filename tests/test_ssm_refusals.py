@@ -1,0 +1,37 @@
+"""CPU: refusals of the state-space operators that are decided on the host before any launch: derivatives they do not have,
+traces, sizes, strides and pointers no kernel can take."""
+import ctypes
+
+import pytest
+import torch
+
+from tests.ssm_cases import scan_inputs
+
+
+def _calls(wrap=lambda v: v, batch=2):
+    """Every entry point on CPU tensors, `wrap` around its main input: without a refusal before it, each ends at "no CPU fallback"."""
+    from vit_amd import ssm
+    s = scan_inputs(4, torch.float32, batch, 5, 4, 8, 2, 16, state=True)
+    t = {k: v[:, 0] if k in ("x", "dt", "Bm", "Cm") else v for k, v in s.items()}
+    x, w, e = torch.ones(batch, 5, 8), torch.ones(8, 4), torch.ones(8)
+    return {
+        "causal_conv": lambda: ssm.causal_conv(wrap(x), w),
+        "causal_conv_step": lambda: ssm.causal_conv_step(wrap(x[:, 0]), w, None, torch.zeros(batch, 3, 8)),
+        "selective_scan": lambda: ssm.selective_scan(wrap(s["x"]), s["dt"], s["A"], s["Bm"], s["Cm"]),
+        "selective_scan_step": lambda: ssm.selective_scan_step(wrap(t["x"]), t["dt"], t["A"], t["Bm"], t["Cm"], s["state"]),
+        "sandwich_norm": lambda: ssm.sandwich_norm(wrap(x), x, e, None, e, None),
+    }
+
+
+NAMES = ("causal_conv", "causal_conv_step", "selective_scan", "selective_scan_step", "sandwich_norm")
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode_is_refused(name):
+    """A dual tensor does not require grad; without a refusal its tangent would be lost, which reads as zero."""
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level(), torch.no_grad():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            _calls(lambda v: forward_ad.make_dual(v, torch.ones_like(v)))[name]()
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        _calls()[name]()

@@ -43,3 +43,18 @@ def test_gate_gradient_is_rounded_once(dev, shape):
     leaf["z"].requires_grad_()
     (dz,) = torch.autograd.grad(_call(ssm, leaf), [leaf["z"]], dy.to(dev))
     _within("dz", dz, want, bound + 1e-30)
+
+
+def test_function_transforms_are_refused(dev):
+    """torch.func's wrappers hold no memory a kernel could read: an error, never a result without its derivative."""
+    from vit_amd import ssm
+    x, w = torch.randn(2, 5, 8, device=dev), torch.randn(8, 4, device=dev)
+    f = lambda v: ssm.causal_conv(v, w)  # noqa: E731
+    for call in (lambda: torch.func.jvp(f, (x,), (x,)), lambda: torch.func.grad(lambda v: f(v).sum())(x), lambda: torch.func.vmap(f)(x[None])):
+        with pytest.raises(RuntimeError):
+            call()
+    with torch.autograd.forward_ad.dual_level():       # a tangent that arrives with the gradient
+        y = ssm.causal_conv(x.clone().requires_grad_(), w)
+        dy = torch.autograd.forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.backward(y, dy)

@@ -44,9 +44,16 @@ void check_lengths(const Tensor& t, int64_t B, const char* op) {
   TORCH_CHECK_VALUE(!t.defined() || (t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == B && t.is_contiguous()), op,
                     ": lengths must be contiguous int32 [", B, "], got ", t.scalar_type(), " ", t.sizes());
 }
+// (a result of a kernel has no tangent, which reads as a tangent of zero)
+void no_tangent(const char* op, const Tensor& t) {
+  TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), op, ": no forward-mode derivatives (torch.autograd.forward_ad)");
+}
 void check_gpu(const char* op, std::initializer_list<Tensor> ts) {
   const at::Device dev = ts.begin()->device();
-  for (const Tensor& t : ts) TORCH_CHECK_VALUE(!t.defined() || t.device() == dev, op, ": tensors on ", dev, " and ", t.device());
+  for (const Tensor& t : ts) {
+    TORCH_CHECK_VALUE(!t.defined() || t.device() == dev, op, ": tensors on ", dev, " and ", t.device());
+    no_tangent(op, t);
+  }
   TORCH_CHECK(dev.is_cuda(), "vit_amd ops run only on the GPU (HIP); got a CPU tensor. There is no CPU fallback.");
 }
 int size(int64_t n, const char* op) {
@@ -70,7 +77,10 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
     if (t.defined() && t.requires_grad()) return true;
   return false;
 }
-void first_order(const char* op) { TORCH_CHECK(!at::GradMode::is_enabled(), op, ": no second derivatives (create_graph=True)"); }
+void first_order(const char* op, const variable_list& g) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), op, ": no second derivatives (create_graph=True)");
+  for (const Tensor& t : g) no_tangent(op, t);
+}
 // a state that a kernel advanced in place: a graph that saved it must notice
 void advanced(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -114,7 +124,7 @@ struct Conv : torch::autograd::Function<Conv> {
     return {out.first};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    first_order("causal_conv");
+    first_order("causal_conv", g);
     const auto s = ctx->get_saved_variables();
     const Tensor &x = s[0], &w = s[1], &bias = s[2], &state = s[3], &lengths = s[4];
     const c10::DeviceGuard guard(x.device());
@@ -229,7 +239,7 @@ struct Scan : torch::autograd::Function<Scan> {
     return {o.y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    first_order("selective_scan");
+    first_order("selective_scan", g);
     const auto s = ctx->get_saved_variables();
     const Tensor &x = s[0], &dt = s[1], &A = s[2], &Bm = s[3], &Cm = s[4], &D = s[5], &z = s[6], &dt_bias = s[7], &lengths = s[8], &v = s[9], &states = s[10];
     const c10::DeviceGuard guard(x.device());
@@ -349,7 +359,7 @@ struct Sandwich : torch::autograd::Function<Sandwich> {
     return {out.first, out.second};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    first_order("sandwich_norm");
+    first_order("sandwich_norm", g);
     const auto s = ctx->get_saved_variables();
     const Tensor &residual = s[0], &y = s[1], &pw = s[2], &pb = s[3], &nw = s[4], &nb = s[5], &gate = s[6], &stats = s[7];
     const c10::DeviceGuard guard(y.device());
