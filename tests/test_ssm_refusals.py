@@ -35,3 +35,13 @@ def test_forward_mode_is_refused(name):
             _calls(lambda v: forward_ad.make_dual(v, torch.ones_like(v)))[name]()
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         _calls()[name]()
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_traces_are_refused(name):
+    """torch.jit.trace records torch operations: of these calls it would keep an uninitialised result and no kernel."""
+    def run(v):
+        return _calls(lambda x: x * v)[name]()
+
+    with pytest.raises(RuntimeError, match="torch.jit.trace"):
+        torch.jit.trace(run, torch.ones(()))

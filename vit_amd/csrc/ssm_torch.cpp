@@ -9,6 +9,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "../../include/rvit.h"
 
@@ -49,6 +50,8 @@ void no_tangent(const char* op, const Tensor& t) {
   TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), op, ": no forward-mode derivatives (torch.autograd.forward_ad)");
 }
 void check_gpu(const char* op, std::initializer_list<Tensor> ts) {
+  // (a trace holds torch operations: the allocation of a result, and nothing that fills it)
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), op, ": torch.jit.trace cannot record it");
   const at::Device dev = ts.begin()->device();
   for (const Tensor& t : ts) {
     TORCH_CHECK_VALUE(!t.defined() || t.device() == dev, op, ": tensors on ", dev, " and ", t.device());

@@ -5,9 +5,9 @@ through the torch binding csrc/ssm_torch.cpp.  The temporal encoder's `model_typ
 Tensors live on one GPU; launches go to the current stream of that GPU.  Activations are bf16 or fp32, per-channel and
 per-head parameters and kept scan states fp32.  Sums, states and statistics are fp32 or wider whatever the inputs.  Results do
 not depend on the order in which workgroups run.  First derivatives in reverse mode only: dual tensors (forward mode) and
-create_graph=True raise RuntimeError.  Wrong shapes, types and devices raise ValueError, a CPU tensor RuntimeError: there is no
-CPU path.  Calls can be captured into graphs, training steps with their backward passes too (these only while no eager autograd
-graph of the same leaves is alive, as for every torch operation)."""
+create_graph=True raise RuntimeError, as does torch.jit.trace.  Wrong shapes, types and devices raise ValueError, a CPU tensor
+RuntimeError: there is no CPU path.  Calls can be captured into graphs, training steps with their backward passes too (these
+only while no eager autograd graph of the same leaves is alive, as for every torch operation)."""
 from __future__ import annotations
 
 import os
