@@ -45,3 +45,30 @@ def test_traces_are_refused(name):
 
     with pytest.raises(RuntimeError, match="torch.jit.trace"):
         torch.jit.trace(run, torch.ones(()))
+
+
+@pytest.mark.parametrize("which", ["x", "w", "b", "state"])
+def test_a_convolution_step_drops_no_gradient(which):
+    """In grad mode an input that requires grad is an error, not a result without its gradient; nothing is written into a leaf."""
+    from vit_amd import ssm
+    t = dict(x=torch.ones(2, 8), w=torch.ones(8, 4), b=torch.ones(8), state=torch.zeros(2, 3, 8))
+    t[which].requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ssm.causal_conv_step(t["x"], t["w"], t["b"], t["state"])
+    with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
+        ssm.causal_conv_step(t["x"], t["w"], t["b"], t["state"])
+
+
+@pytest.mark.parametrize("which", ["x", "dt", "A", "Bm", "Cm", "state", "D", "z", "dt_bias"])
+def test_a_scan_step_drops_no_gradient(which):
+    from vit_amd import ssm
+    s = scan_inputs(4, torch.float32, 2, None, 4, 8, 2, 16, state=True, slices=False)
+    s[which].requires_grad_()
+
+    def call():
+        return ssm.selective_scan_step(*(s[k] for k in ("x", "dt", "A", "Bm", "Cm", "state")), D=s["D"], z=s["z"], dt_bias=s["dt_bias"])
+
+    with pytest.raises(RuntimeError, match="no gradient"):
+        call()
+    with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
+        call()

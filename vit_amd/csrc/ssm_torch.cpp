@@ -80,6 +80,9 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
     if (t.defined() && t.requires_grad()) return true;
   return false;
 }
+void no_gradient(const char* op, std::initializer_list<Tensor> ts) {
+  TORCH_CHECK(!wants_grad(ts), op, ": has no gradient, and an input requires one (torch.no_grad(), or detach it)");
+}
 void first_order(const char* op, const variable_list& g) {
   TORCH_CHECK(!at::GradMode::is_enabled(), op, ": no second derivatives (create_graph=True)");
   for (const Tensor& t : g) no_tangent(op, t);
@@ -171,6 +174,7 @@ Tensor conv_step(Tensor x, const Tensor& w, const Opt& bias_, const Tensor& stat
   const Tensor bias = get(bias_);
   conv_shapes("causal_conv_step", x, w, bias, true);
   check_like(state, x, {x.size(0), w.size(1) - 1, x.size(1)}, "causal_conv_step", "state");
+  no_gradient("causal_conv_step", {x, w, bias, state});
   check_gpu("causal_conv_step", {x, w, bias, state});
   const c10::DeviceGuard guard(x.device());
   x = packed(x, 1);
@@ -297,6 +301,7 @@ Tensor scan_step(Tensor x, Tensor dt, const Tensor& A, Tensor Bm, Tensor Cm, con
   Tensor z = get(z_);
   scan_shapes("selective_scan_step", x, dt, A, Bm, Cm, D, z, dt_bias, true);
   check_f32(state, {x.size(0), x.size(1), x.size(2), Bm.size(2)}, "selective_scan_step", "state");
+  no_gradient("selective_scan_step", {x, dt, A, Bm, Cm, D, z, dt_bias, state});
   check_gpu("selective_scan_step", {x, dt, A, Bm, Cm, D, z, dt_bias, state});
   const c10::DeviceGuard guard(x.device());
   x = packed(x, 2);

@@ -55,7 +55,8 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
 
 def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], state: torch.Tensor, *,
                      activation: Optional[str] = None) -> torch.Tensor:
-    """causal_conv for one token: x [B,C], state [B,K-1,C] (advances in place); returns [B,C].  No gradient."""
+    """causal_conv for one token: x [B,C], state [B,K-1,C] (advances in place); returns [B,C].  No gradient: in grad
+    mode an input that requires one raises RuntimeError."""
     args = (x, weight, bias, state, _silu(activation))
     fn = (_ext or _load()).conv_step
     return fn(*args) if ops._PROF is None else _profiled("ssm_conv_step", 2 * x.numel() * weight.shape[1], (x, x, state, state), fn, *args)
@@ -91,7 +92,7 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: 
                         D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
                         dt_bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """selective_scan for one token: x, z [B,H,P], dt [B,H], Bm, Cm [B,G,N], state fp32 [B,H,P,N] (advances in place); returns
-    [B,H,P].  No gradient."""
+    [B,H,P].  No gradient: in grad mode an input that requires one raises RuntimeError."""
     args = (x, dt, A, Bm, Cm, state, D, z, dt_bias)
     fn = (_ext or _load()).scan_step
     return fn(*args) if ops._PROF is None else _profiled("ssm_scan_step", x.numel() * (5 * Bm.shape[-1] + 6), (x, dt, Bm, Cm, z, x, state, state),
