@@ -58,3 +58,46 @@ def test_function_transforms_are_refused(dev):
         dy = torch.autograd.forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
         with pytest.raises(RuntimeError, match="forward-mode"):
             torch.autograd.backward(y, dy)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("low", [float("-inf"), "min"])
+def test_tokens_masked_through_dt_do_nothing(dev, low, dtype):
+    """dt of -infinity or of the type's lowest value: softplus is zero, the state stays bit for bit, and what starts from nothing
+    stays nothing."""
+    from vit_amd import ssm
+    dt = DTYPES[dtype]
+    low = torch.finfo(dt).min if low == "min" else low
+    B, T, H, P, G, N = 2, 100, 4, 24, 2, 20
+    s = scan_inputs(70, dt, B, T, H, P, G, N)
+    s["x"].mul_(64.0)
+    s["D"] = s["z"] = None
+    s["dt"].fill_(low)
+    d = to(s, dev)
+    y, end = _call(ssm, d, return_state=True)
+    assert float(y.abs().max()) == 0.0 and float(end.abs().max()) == 0.0
+    state = torch.randn(B, H, P, N, device=dev)
+    _, end = _call(ssm, dict(d, state=state), return_state=True)
+    assert torch.equal(end, state)
+    for start in (state, torch.zeros_like(state)):
+        moved = start.clone()
+        ssm.selective_scan_step(d["x"][:, 0], d["dt"][:, 0], d["A"], d["Bm"][:, 0], d["Cm"][:, 0], moved, dt_bias=d["dt_bias"])
+        assert torch.equal(moved, start)
+    # some of the tokens masked: values and gradients
+    s = scan_inputs(71, dt, B, T, H, P, G, N, state=True)
+    s["dt"][:, 10:80:3] = low
+    s["dt"][1, 64:] = low
+    want_in = leaves64(s)
+    wy, wend = ref.selective_scan(**want_in)
+    names = [k for k in want_in if want_in[k] is not None]
+    g = torch.Generator().manual_seed(72)
+    dy, dend = randn(g, *wy.shape, dtype=dt), randn(g, *wend.shape)
+    want = torch.autograd.grad([wy, wend], [want_in[k] for k in names], [dy.double(), dend.double()])
+    leaf = {k: v.requires_grad_() for k, v in to(s, dev).items()}
+    y, end = _call(ssm, leaf, return_state=True)
+    close("y", y, wy)
+    close("end", end, wend)
+    for k, a, b in zip(names, torch.autograd.grad([y, end], [leaf[k] for k in names], [dy.to(dev), dend.to(dev)]), want):
+        close("d" + k, a, b)
+        if k == "dt":
+            assert float(a[s["dt"].to(dev) == low].abs().max()) == 0.0

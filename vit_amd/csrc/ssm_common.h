@@ -287,9 +287,10 @@ __device__ __forceinline__ float ssm_exp(float x) {
 // much smaller
 __device__ __forceinline__ float ssm_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + ssm_exp2(x * -1.44269502f)); }
 // max(x, 0) + log(1 + e), e = exp(-|x|): with s = e / (2 + e) <= 1/3 the logarithm is 2 atanh(s) = 2 (s + s^3 / 3 + s^5 / 5 ..);
-// the terms up to s^15 leave 2e-9 of it, and small e keep their relative precision (steps of 1e-3 and less are common)
+// the terms up to s^15 leave 2e-9 of it, and small e keep their relative precision (steps of 1e-3 and less are common).  Below
+// -87 the result is under the type's normal range: zero, so that tokens masked by -infinity or the type's lowest value do nothing
 __device__ __forceinline__ float ssm_softplus(float x) {
-  const float e = ssm_exp(-fminf(fabsf(x), 87.f));
+  const float e = x < -87.f ? 0.f : ssm_exp(-fminf(fabsf(x), 87.f));
   const float s = e * __builtin_amdgcn_rcpf(2.0f + e), u = s * s;
   float p = fmaf(u, 1.0f / 15.0f, 1.0f / 13.0f);
   p = fmaf(p, u, 1.0f / 11.0f);
