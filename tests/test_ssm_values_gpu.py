@@ -101,3 +101,48 @@ def test_tokens_masked_through_dt_do_nothing(dev, low, dtype):
         close("d" + k, a, b)
         if k == "dt":
             assert float(a[s["dt"].to(dev) == low].abs().max()) == 0.0
+
+
+def test_fp32_gates_over_their_range(dev):
+    """silu of fp32 values from -85 to 85, value by value: exp(-x) to 1.5 units in the last place (v_exp_f32: one, and its correction's
+    rounding), the sum with 1 (0.5), v_rcp_f32 (one) and the product (0.5): 3.5, held to 4 units of 2^-23.  silu'(x) = s + x s (1 - s)
+    where x < -2: s to 3 units, twice in its second term, and four roundings: 8 of its parts' sizes, which are within 2.2 of its
+    own there and further out within 1.1: 8 of the parts."""
+    from vit_amd import ssm
+    x = torch.linspace(-85, 85, 4096)
+    x64 = x.double()
+    sg = torch.sigmoid(x64)
+    want = x64 * sg
+    w = torch.tensor([0.0, 1.0]).repeat(4096, 1)
+    xd = x.to(dev).view(1, 1, -1).requires_grad_()
+    y = ssm.causal_conv(xd, w.to(dev), activation="silu")
+    tiny = 1e-36      # (below, results have left the normal range's neighbourhood)
+    _within("conv", y[0, 0], want, 4 * 2.0 ** -23 * want.abs() + tiny)
+    step = ssm.causal_conv_step(xd[0].detach(), w.to(dev), None, torch.zeros(1, 1, 4096, device=dev), activation="silu")
+    _within("step", step[0], want, 4 * 2.0 ** -23 * want.abs() + tiny)
+    slope, parts = sg + x64 * sg * (1 - sg), sg + x64.abs() * sg * (1 - sg)
+    (dx,) = torch.autograd.grad(y.sum(), [xd])
+    at = x64 < -2
+    _within("conv dx", dx[0, 0].cpu()[at], slope[at], 8 * 2.0 ** -23 * parts[at] + tiny)
+    # the scan's gate: B = 0 and D = 1 make v = x = 1
+    H, P = 64, 64
+    z = x.to(dev).view(1, 1, H, P).requires_grad_()
+    one, none = torch.ones(1, 1, H, P, device=dev), torch.zeros(1, 1, 1, 8, device=dev)
+    per = lambda v: torch.full((H,), v, device=dev)  # noqa: E731
+    y = ssm.selective_scan(one, torch.zeros(1, 1, H, device=dev), per(-1.0), none, none, D=per(1.0), z=z)
+    _within("scan", y.reshape(-1), want, 4 * 2.0 ** -23 * want.abs() + tiny)
+    (dz,) = torch.autograd.grad(y.sum(), [z])
+    _within("scan dz", dz.reshape(-1).cpu()[at], slope[at], 8 * 2.0 ** -23 * parts[at] + tiny)
+    step = ssm.selective_scan_step(one[:, 0], torch.zeros(1, H, device=dev), per(-1.0), none[:, 0], none[:, 0], torch.zeros(1, H, P, 8, device=dev), D=per(1.0),
+                                   z=z[:, 0].detach())
+    _within("scan step", step.reshape(-1), want, 4 * 2.0 ** -23 * want.abs() + tiny)
+
+
+def test_gates_at_the_ends_of_the_type(dev):
+    """Far from zero silu is x or nothing; NaN stays NaN, and nothing else becomes one."""
+    from vit_amd import ssm
+    w = torch.tensor([[0.0, 1.0]], device=dev)
+    for dt in DTYPES.values():
+        x = torch.tensor([-3e38, -1e30, -1000.0, -104.0, -89.0, -88.0, 0.0, 89.0, 1000.0, 1e30, 3e38, float("inf"), float("nan")], device=dev, dtype=dt)
+        y = torch.cat([ssm.causal_conv(v.view(1, 1, 1), w, activation="silu").view(1) for v in x])
+        assert float(y[:6].abs().max()) <= 1e-35 and float(y[6]) == 0.0 and torch.equal(y[7:12], x[7:12]) and bool(torch.isnan(y[12])), y

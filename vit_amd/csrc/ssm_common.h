@@ -283,9 +283,15 @@ __device__ __forceinline__ float ssm_exp(float x) {
   const float e = ssm_exp2(t);
   return fmaf(e, lo * 0.693147182f, e);
 }
-// 1 / (1 + exp(-x)); exp(-x) is good to |x| 2^-24, which the sum with 1 hides where x > 0, and where x < 0 the result is that
-// much smaller
-__device__ __forceinline__ float ssm_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + ssm_exp2(x * -1.44269502f)); }
+// 1 / (1 + exp(-x)) of calls on T.  bf16: exp(-x) good to |x| 2^-24 of itself, far below the 2^-8 of their results.  fp32: to 3 units
+// in the last place (exp(-x) 1.5, the sum 0.5, the reciprocal 1); under exp(-88) zero.  NaN passes through (selects, no minima).
+template <typename T> __device__ __forceinline__ float ssm_sigmoid(float x) {
+  if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(1.0f + ssm_exp2(x * -1.44269502f));
+  float y = x > 87.f ? -87.f : -x;
+  y = y > 88.f ? 88.f : y;
+  const float s = __builtin_amdgcn_rcpf(1.0f + ssm_exp(y));
+  return x < -88.f ? 0.f : s;
+}
 // max(x, 0) + log(1 + e), e = exp(-|x|): with s = e / (2 + e) <= 1/3 the logarithm is 2 atanh(s) = 2 (s + s^3 / 3 + s^5 / 5 ..);
 // the terms up to s^15 leave 2e-9 of it, and small e keep their relative precision (steps of 1e-3 and less are common).  Below
 // -87 the result is under the type's normal range: zero, so that tokens masked by -infinity or the type's lowest value do nothing

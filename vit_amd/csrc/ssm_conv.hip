@@ -108,7 +108,7 @@ __global__ __launch_bounds__(256) void ssm_conv_fwd_kernel(SsmConvArgs a) {
         u[j] = bias[j];
 #pragma unroll
         for (int k = 0; k < K; ++k) u[j] = fmaf(w[k][j], win[k][j], u[j]);
-        if (a.silu) u[j] *= ssm_sigmoid(u[j]);
+        if (a.silu) u[j] *= ssm_sigmoid<T>(u[j]);
 #pragma unroll
         for (int k = 0; k + 1 < K; ++k) win[k][j] = win[k + 1][j];
       }
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(256, V >= 4 && K >= 5 ? 3 : 4) void ssm_conv_bwd_ke
             float u = bias[j];
 #pragma unroll
             for (int k = 0; k < K; ++k) u = fmaf(w[k][j], win[at(k)][j], u);
-            const float sg = ssm_sigmoid(u);
+            const float sg = ssm_sigmoid<T>(u);
             g[j] = t < len ? g[j] * (sg + u * sg * (1.f - sg)) : 0.f;
           }
           du[at(K - 1)][j] = g[j];
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(256) void ssm_conv_step_kernel(SsmConvArgs a) {
     u[j] = bias[j];
 #pragma unroll
     for (int k = 0; k < K; ++k) u[j] = fmaf(w[k][j], win[k][j], u[j]);
-    if (a.silu) u[j] *= ssm_sigmoid(u[j]);
+    if (a.silu) u[j] *= ssm_sigmoid<T>(u[j]);
   }
 #pragma unroll
   for (int k = 0; k < K - 1; ++k) stv<T, V>(st + (long)k * a.C, win[k + 1]);

@@ -246,7 +246,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_
             float zv[4];
             zr[tt].get(zv);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) out[i] *= zv[i] * ssm_sigmoid(zv[i]);
+            for (int i = 0; i < 4; ++i) out[i] *= zv[i] * ssm_sigmoid<T>(zv[i]);
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {          // (a last chunk's rows behind the end)
@@ -376,7 +376,7 @@ __global__ __launch_bounds__(256) void ssm_scan_step_kernel(SsmStepArgs a) {
     for (int o = 1; o < LN; o <<= 1) acc += __shfl_xor(acc, o, 64);
     if (ln == 0) {
       float v = acc + Dh * xv;
-      if (z) { const float zv = ssm_ld(z + p); v *= zv * ssm_sigmoid(zv); }
+      if (z) { const float zv = ssm_ld(z + p); v *= zv * ssm_sigmoid<T>(zv); }
       ssm_st(y + p, v);
     }
   }

@@ -115,7 +115,7 @@ __global__ __launch_bounds__(256, 2) void ssm_scan_bwd_state_kernel(SsmBwdArgs a
       if (z) zr[i].get(zv);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (z) v[j] *= zv[j] * ssm_sigmoid(zv[j]);
+        if (z) v[j] *= zv[j] * ssm_sigmoid<T>(zv[j]);
         if (t >= live || p >= pw) v[j] = 0.f;
       }
       *reinterpret_cast<float4*>(Vs + t * PV + p) = make_float4(v[0], v[1], v[2], v[3]);
@@ -423,7 +423,7 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
             vr[i].get(vv);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const float sg = ssm_sigmoid(zv[j]), zs = zv[j] * sg;
+              const float sg = ssm_sigmoid<T>(zv[j]), zs = zv[j] * sg;
               dzv[j] = dv[j] * vv[j] * (sg + zs * (1.f - sg));
               dv[j] *= zs;
             }
@@ -455,7 +455,7 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
           slo[lane] = (float)(l2 - (double)hi);
           sw[lane] = ssm_exp2((float)(end - l2));
           se[lane] = ssm_exp2(hi);
-          ssg[lane] = ssm_sigmoid(raw);
+          ssg[lane] = ssm_sigmoid<float>(raw);
         }
         if constexpr (L::DS_LDS) {
           int tid = threadIdx.x;
