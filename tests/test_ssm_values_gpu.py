@@ -146,3 +146,38 @@ def test_gates_at_the_ends_of_the_type(dev):
         x = torch.tensor([-3e38, -1e30, -1000.0, -104.0, -89.0, -88.0, 0.0, 89.0, 1000.0, 1e30, 3e38, float("inf"), float("nan")], device=dev, dtype=dt)
         y = torch.cat([ssm.causal_conv(v.view(1, 1, 1), w, activation="silu").view(1) for v in x])
         assert float(y[:6].abs().max()) <= 1e-35 and float(y[6]) == 0.0 and torch.equal(y[7:12], x[7:12]) and bool(torch.isnan(y[12])), y
+
+
+def test_fp32_decays_keep_their_low_bits(dev):
+    """y_t = exp(L_t) of a state of one, L_t the sum of 64 exact log decays down to -45: v_exp_f32 one unit in the last place, the low
+    part's correction a half, held to two (2^-22).  (Steps of 30 and more: softplus adds nothing, so the sums are known exactly.)
+    A step's factor likewise; the end of five chunks is a product of five such factors and its four roundings."""
+    from vit_amd import ssm
+    T, H = 64 * 5, 16
+    g = torch.Generator().manual_seed(80)
+    dt = 30.0 + 4.0 * torch.rand(1, T, H, generator=g)
+    A = -0.02 * (1 + 0.1 * torch.rand(H, generator=g))
+    L = (dt.double() * A.double()).cumsum(1)
+    zero, one = torch.zeros(1, T, H, 1, device=dev), torch.ones(1, T, 1, 1, device=dev)
+    for t in (1, 33, 64):
+        y, end = ssm.selective_scan(zero[:, :t], dt[:, :t].to(dev), A.to(dev), one[:, :t], one[:, :t], state=torch.ones(1, H, 1, 1, device=dev), return_state=True)
+        want = torch.exp(L[:, :t])
+        _within("y", y[..., 0], want, 2.0 ** -22 * want)
+        _within("end", end[..., 0, 0], want[:, -1], 2.0 ** -22 * want[:, -1])
+    # (the head with the slowest decay alone: five chunks stay inside the type)
+    slow = A / 8
+    L = (dt.double() * slow.double()).cumsum(1)
+    _, end = ssm.selective_scan(zero, dt.to(dev), slow.to(dev), one, one, state=torch.ones(1, H, 1, 1, device=dev), return_state=True)
+    want = torch.exp(L[:, -1])
+    _within("end of five", end[..., 0, 0], want, (5 * 2.0 ** -22 + 4 * 2.0 ** -24) * want)
+    # what token 0 of 64 leaves behind: d exp(L_63 - L_0) x B
+    x = torch.zeros(1, 64, H, 1, device=dev)
+    x[:, 0] = 1.0
+    L = (dt[:, :64].double() * A.double()).cumsum(1)
+    _, end = ssm.selective_scan(x, dt[:, :64].to(dev), A.to(dev), one[:, :64], one[:, :64], return_state=True)
+    want = dt[:, 0].double() * torch.exp(L[:, 63] - L[:, 0])
+    _within("left behind", end[..., 0, 0], want, 2.0 ** -22 * want)
+    st = torch.ones(1, H, 1, 1, device=dev)
+    ssm.selective_scan_step(zero[:, 0], 20 * dt[:, 0].to(dev), A.to(dev), one[:, 0], one[:, 0], st)
+    want = torch.exp((20 * dt[:, 0]).double() * A.double())
+    _within("step", st[..., 0, 0], want, 2.0 ** -22 * want)

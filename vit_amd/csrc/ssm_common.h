@@ -314,6 +314,13 @@ __device__ __forceinline__ double ssm_log_decay(float d, double A2) {
   return l < -1e5 ? -1e5 : l;
 }
 
+// 2^l of a sum of log decays (at most 0, but for a positive A) to two units in the last place: fp32's rounding of l, |l| 2^-25, is
+// made up for to first order (a result outside the type is infinite or zero as it is)
+__device__ __forceinline__ float ssm_decay(double l) {
+  const float hi = (float)l, e = ssm_exp2(hi);
+  return fabsf(hi) < 128.f ? fmaf(e, (float)(l - (double)hi) * 0.693147182f, e) : e;
+}
+
 // A ROWS x COLS image on its way from global memory (row stride `ld`) to LDS through the registers of a workgroup: load() is
 // issued a chunk ahead of store(), so that its latency passes under the products between.  What lies outside rows x cols is
 // written as zero: rows behind a sequence's end never enter a product, whatever they hold.  load() takes addresses inside

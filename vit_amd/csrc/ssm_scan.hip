@@ -148,8 +148,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_
     sd[lane] = d;
     sd[Q + lane] = hi;
     sd[2 * Q + lane] = (float)(l2 - (double)hi);
-    sd[3 * Q + lane] = ssm_exp2((float)(end - l2)) * d;
-    sd[4 * Q + lane] = ssm_exp2(hi);
+    sd[3 * Q + lane] = ssm_decay(end - l2) * d;
+    sd[4 * Q + lane] = ssm_decay(l2);
     total += end;
   };
   const int c0 = seg * a.seg_chunks, c1 = min(a.nchunks, c0 + a.seg_chunks);
@@ -326,14 +326,14 @@ __global__ __launch_bounds__(64) void ssm_join_kernel(float* seg_state, const do
       f[j] = 0.f;
       if (j0 + j < nseg - 1) {      // (of the last one nothing is needed)
         own[j] = st[(j0 + j) * step];
-        f[j] = (float)dec[(j0 + j) * sb];
+        f[j] = ssm_decay(dec[(j0 + j) * sb]);
       }
     }
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j)
       if (j0 + j < nseg) {
         st[(j0 + j) * step] = run;
-        run = ssm_exp2(f[j]) * run + own[j];
+        run = f[j] * run + own[j];
       }
   }
 }
@@ -347,7 +347,7 @@ __global__ __launch_bounds__(256) void ssm_scan_step_kernel(SsmStepArgs a) {
   const int h = id % a.H, b = id / a.H;
   const int g = h / (a.H / a.G);
   const float d = ssm_softplus(ssm_ld((const T*)a.dt + b * a.sdb + h) + (a.dt_bias ? a.dt_bias[h] : 0.f));
-  const float f = ssm_exp2((float)ssm_log_decay(d, (double)a.A[h] * 1.4426950408889634));
+  const float f = ssm_decay(ssm_log_decay(d, (double)a.A[h] * 1.4426950408889634));
   const T* x = (const T*)a.x + b * a.sxb + (long)h * a.P;
   const T* Bm = (const T*)a.Bm + b * a.sbb + (long)g * a.N;
   const T* Cm = (const T*)a.Cm + b * a.scb + (long)g * a.N;

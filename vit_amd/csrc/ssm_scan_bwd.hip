@@ -85,7 +85,7 @@ __global__ __launch_bounds__(256, 2) void ssm_scan_bwd_state_kernel(SsmBwdArgs a
   auto decay = [&](T raw, int ch) {
     const float d = ch * Q + lane < len ? ssm_softplus((float)raw + bias) : 0.f;
     const double l2 = ssm_scan64(ssm_log_decay(d, A2));
-    decays[(ch & 1) * Q + lane] = chunk_sign(ch - 1) * ssm_exp2((float)l2);
+    decays[(ch & 1) * Q + lane] = chunk_sign(ch - 1) * ssm_decay(l2);
     total += ssm_last_lane(l2);
   };
   const int c0 = seg * f.seg_chunks, cl = min(min(f.nchunks, c0 + f.seg_chunks), (len + Q - 1) / Q);
@@ -453,8 +453,8 @@ __global__ __launch_bounds__(512, 2) void ssm_scan_bwd_chunk_kernel(SsmBwdArgs a
           sd[lane] = d;
           shi[lane] = hi;
           slo[lane] = (float)(l2 - (double)hi);
-          sw[lane] = ssm_exp2((float)(end - l2));
-          se[lane] = ssm_exp2(hi);
+          sw[lane] = ssm_decay(end - l2);
+          se[lane] = ssm_decay(l2);
           ssg[lane] = ssm_sigmoid<float>(raw);
         }
         if constexpr (L::DS_LDS) {
