@@ -72,3 +72,19 @@ def test_a_scan_step_drops_no_gradient(which):
         call()
     with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
         call()
+
+
+SCAN = [64, 1, 1, 64, 1, 1, 64, 64, 1, 1, 64, 1, 1, None, None, 0, 0, None, None, None, 64, None, None, None]
+
+
+def _scan_fwd(lib, *, args=SCAN, ws=(None, 0), dtype=1, sizes=(1, 64, 1, 64, 1, 64)):
+    return lib.rvit_ssm_scan_fwd(*args, *ws, dtype, *sizes, None)
+
+
+def test_no_tokens_still_need_their_decay():
+    """A scan of no tokens reads A on its way to the state it returns: null is refused before a launch."""
+    from vit_amd import _lib
+    lib = _lib.load()
+    args = list(SCAN)
+    args[6] = None
+    assert _scan_fwd(lib, args=args, sizes=(1, 0, 1, 64, 1, 64)) == -1 and b"null" in lib.rvit_last_error()

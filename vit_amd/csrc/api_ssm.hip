@@ -55,7 +55,7 @@ int shape(SsmScanArgs& a, int dtype, int B, int T, int H, int P, int G, int N) {
 int inputs(SsmScanArgs& a, int dtype, const void* x, int64_t sxb, int64_t sxt, const void* dt, int64_t sdb, int64_t sdt, const float* A,
            const void* Bm, int64_t sbb, int64_t sbt, const void* Cm, int64_t scb, int64_t sct, const float* D, const void* z, int64_t szb,
            int64_t szt, const float* dt_bias, const int* lengths) {
-  RVIT_CHECK_ARG(a.T == 0 || (x && dt && A && Bm && Cm), "ssm_scan: null pointer");
+  RVIT_CHECK_ARG(A && (a.T == 0 || (x && dt && Bm && Cm)), "ssm_scan: null pointer");
   a.x = x; a.dt = dt; a.A = A; a.Bm = Bm; a.Cm = Cm; a.D = D; a.z = z; a.dt_bias = dt_bias; a.lengths = lengths;
   a.sxb = sxb; a.sxt = sxt; a.sdb = sdb; a.sdt = sdt; a.sbb = sbb; a.sbt = sbt; a.scb = scb; a.sct = sct; a.szb = szb; a.szt = szt;
   const int V = 16 / es(dtype);
