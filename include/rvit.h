@@ -640,7 +640,7 @@ int rvit_gru_step_bwd(const float* dout, const float* w_hh_t, const float* w_hh_
 
 /* ---- state-space sequence operators (vit_amd/ssm.py; the temporal encoder's model_type='ssm') ----------------------------
  * Short causal convolution per channel: y[t] = act(bias + sum_k w[:, k] x[t - K + 1 + k]), 2 <= K <= 6, act = SiLU (silu != 0)
- * or none.  x [B,T,C] (strides sxb, sxt in elements, channels packed), w fp32 [C,K], bias fp32 [C] or null; `state`
+ * or none.  x [B,T,C] (strides sxb, sxt in elements, none negative, channels packed), w fp32 [C,K], bias fp32 [C] or null; `state`
  * [B,K-1,C] holds the inputs before the first token (null: zero), state_out receives the last K-1 before the end (may be null,
  * may not be `state`).  lengths int32 [B] or null: sample b ends after lengths[b] tokens (clamped to 0..T); outputs and input
  * gradients behind the end are zero, whatever the inputs hold there.  x, y, state of one dtype.  bwd: dw [C,K], dbias [C]
@@ -659,7 +659,7 @@ int rvit_ssm_conv_step(const void* x, int64_t sxb, const float* w, const float* 
 
 /* Selective scan: d = softplus(dt + dt_bias), S_t = exp(d_t A) S_{t-1} + d_t x_t B_t^T, y_t = (S_t C_t + D x_t) silu(z_t).
  * x, z, y [B,T,H,P]; dt [B,T,H]; Bm, Cm [B,T,G,N] (shared by the H / G heads of a group), one dtype; A, D, dt_bias fp32 [H];
- * states fp32 [B,H,P,N], 1 <= N <= 128.  Inputs have strides per sample and token in elements ([H,P], [G,N], [H] packed);
+ * states fp32 [B,H,P,N], 1 <= N <= 128.  Inputs have strides per sample and token in elements, none negative ([H,P], [G,N], [H] packed);
  * outputs are packed.  D, z, dt_bias, state0, lengths, state_out may be null.  lengths as above: the returned state is the one
  * behind the last token of each sample.  Training passes v (fp32, [B,T,H,P]; only with z) and states (fp32, state_floats of
  * rvit_ssm_scan_plan), both read by bwd.  Workspaces: fwd_bytes / bwd_bytes of rvit_ssm_scan_plan, 16-byte aligned.  bwd:

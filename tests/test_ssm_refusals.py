@@ -88,3 +88,31 @@ def test_no_tokens_still_need_their_decay():
     args = list(SCAN)
     args[6] = None
     assert _scan_fwd(lib, args=args, sizes=(1, 0, 1, 64, 1, 64)) == -1 and b"null" in lib.rvit_last_error()
+
+
+@pytest.mark.parametrize("at", [1, 2, 4, 5, 8, 9, 11, 12, 15, 16])
+def test_negative_strides_are_refused(at):
+    """The wide paths take token strides as 32-bit unsigned offsets: a negative one would read 4 GiB further on."""
+    from vit_amd import _lib
+    lib = _lib.load()
+    args = list(SCAN)
+    args[at] = -64
+    assert _scan_fwd(lib, args=args) == -1 and b"stride" in lib.rvit_last_error()
+    bwd = args[:19] + [64, 64, 64, 1, 1, None, 64, 64, 64, 64, 64, None, None, None, None, 64, 1 << 40]
+    assert lib.rvit_ssm_scan_bwd(*bwd, 1, 1, 64, 1, 64, 1, 64, None) == -1 and b"stride" in lib.rvit_last_error()
+
+
+def test_negative_strides_of_the_gradient_and_of_a_convolution():
+    from vit_amd import _lib
+    lib = _lib.load()
+    for syb, syt in ((-1, 64), (64, -1)):
+        bwd = SCAN[:19] + [64, 64, 64, syb, syt, None, 64, 64, 64, 64, 64, None, None, None, None, 64, 1 << 40]
+        assert lib.rvit_ssm_scan_bwd(*bwd, 1, 1, 64, 1, 64, 1, 64, None) == -1 and b"stride" in lib.rvit_last_error()
+        assert lib.rvit_ssm_conv_fwd(64, syb, syt, 64, None, None, None, 64, None, 1, 1, 8, 8, 4, 0, None) == -1 and b"stride" in lib.rvit_last_error()
+        assert lib.rvit_ssm_conv_bwd(64, 64, 8, 64, None, None, None, 64, syb, syt, None, 64, 64, None, None, 64, 1 << 40, 1, 1, 8, 8, 4, 0, None) == -1
+        assert b"stride" in lib.rvit_last_error()
+    for i in (1, 3, 6, 8, 11):
+        step = [64, 1, 64, 1, 64, 64, 1, 64, 1, None, 64, 1, None, 64, 64]
+        step[i] = -1
+        assert lib.rvit_ssm_scan_step(*step, 1, 1, 1, 64, 1, 64, None) == -1 and b"stride" in lib.rvit_last_error(), i
+    assert lib.rvit_ssm_conv_step(64, -1, 64, None, 64, 64, 1, 1, 8, 4, 0, None) == -1 and b"stride" in lib.rvit_last_error()

@@ -11,6 +11,11 @@ int es(int dtype) { return dtype == RVIT_BF16 ? 2 : 4; }
 // Token strides under this fit a 32-bit byte offset over the tokens of a chunk, which the kernels' wide paths use (63 strides
 // of fp32 and a row's columns: 63 * 4 * (2^24 - 1) + 4 * 128 < 2^32); larger ones take the paths with 64-bit offsets.
 constexpr int64_t MOST = 1 << 24;
+bool strides_ok(std::initializer_list<int64_t> s) {      // (unsigned there: none may be negative)
+  for (int64_t v : s)
+    if (v < 0) return false;
+  return true;
+}
 
 // Segments of a sequence.  One workgroup walks a (sample, head, 64 channels), and a compute unit holds two of them; where there
 // are too few to fill the chip the sequence is cut, at the price of a pass that only computes states.
@@ -56,6 +61,7 @@ int inputs(SsmScanArgs& a, int dtype, const void* x, int64_t sxb, int64_t sxt, c
            const void* Bm, int64_t sbb, int64_t sbt, const void* Cm, int64_t scb, int64_t sct, const float* D, const void* z, int64_t szb,
            int64_t szt, const float* dt_bias, const int* lengths) {
   RVIT_CHECK_ARG(A && (a.T == 0 || (x && dt && Bm && Cm)), "ssm_scan: null pointer");
+  RVIT_CHECK_ARG(strides_ok({sxb, sxt, sdb, sdt, sbb, sbt, scb, sct, szb, szt}), "ssm_scan: negative stride");
   a.x = x; a.dt = dt; a.A = A; a.Bm = Bm; a.Cm = Cm; a.D = D; a.z = z; a.dt_bias = dt_bias; a.lengths = lengths;
   a.sxb = sxb; a.sxt = sxt; a.sdb = sdb; a.sdt = sdt; a.sbb = sbb; a.sbt = sbt; a.scb = scb; a.sct = sct; a.szb = szb; a.szt = szt;
   const int V = 16 / es(dtype);
@@ -118,6 +124,7 @@ int rvit_ssm_scan_bwd(const void* x, int64_t sxb, int64_t sxt, const void* dt, i
   if (int e = shape(a.f, dtype, B, T, H, P, G, N)) return e;
   if (int e = inputs(a.f, dtype, x, sxb, sxt, dt, sdb, sdt, A, Bm, sbb, sbt, Cm, scb, sct, D, z, szb, szt, dt_bias, lengths)) return e;
   RVIT_CHECK_ARG(T > 0, "ssm_scan_bwd: no tokens");
+  RVIT_CHECK_ARG(strides_ok({syb, syt}), "ssm_scan_bwd: negative stride");
   RVIT_CHECK_ARG(states && dy && dx && ddt && dA && dB && dC && (!z || (v && dz)), "ssm_scan_bwd: null pointer");
   split_heads(a);
   int64_t need = 0;
@@ -150,6 +157,7 @@ int rvit_ssm_scan_step(const void* x, int64_t sxb, const void* dt, int64_t sdb, 
   SsmScanArgs s = {};
   if (int e = shape(s, dtype, B, 1, H, P, G, N)) return e;
   RVIT_CHECK_ARG(x && dt && A && Bm && Cm && state && y, "ssm_scan_step: null pointer");
+  RVIT_CHECK_ARG(strides_ok({sxb, sdb, sbb, scb, szb}), "ssm_scan_step: negative stride");
   SsmStepArgs a = {};
   a.x = x; a.dt = dt; a.A = A; a.Bm = Bm; a.Cm = Cm; a.D = D; a.z = z; a.dt_bias = dt_bias; a.state = state; a.y = y;
   a.sxb = sxb; a.sdb = sdb; a.sbb = sbb; a.scb = scb; a.szb = szb;
@@ -169,6 +177,7 @@ int conv_args(SsmConvArgs& a, int dtype, const void* x, int64_t sxb, int64_t sxt
   RVIT_CHECK_ARG(B > 0 && T > 0 && C > 0 && K >= 2 && K <= 6, "ssm_conv: bad sizes B=%d T=%d C=%d K=%d (K: 2 .. 6)", B, T, C, K);
   RVIT_CHECK_ARG((int64_t)B * C < (1 << 30) && T < (1 << 28), "ssm_conv: too many rows");
   RVIT_CHECK_ARG(x && w, "ssm_conv: null pointer");
+  RVIT_CHECK_ARG(strides_ok({sxb, sxt}), "ssm_conv: negative stride");
   a.x = x; a.sxb = sxb; a.sxt = sxt; a.w = w; a.bias = bias; a.B = B; a.T = T; a.C = C; a.K = K; a.silu = silu;
   const int V = 16 / es(dtype);
   a.vec = at(x, 16) && at(w, 16) && at(bias, 16) && sxb % V == 0 && sxt % V == 0 && C % V == 0;
@@ -217,6 +226,7 @@ int rvit_ssm_conv_bwd(const void* x, int64_t sxb, int64_t sxt, const float* w, c
                       void* workspace, int64_t workspace_bytes, int dtype, int B, int T, int C, int K, int silu, void* stream) {
   SsmConvArgs a = {};
   if (int e = conv_args(a, dtype, x, sxb, sxt, w, bias, B, T, C, K, silu)) return e;
+  RVIT_CHECK_ARG(strides_ok({syb, syt}), "ssm_conv_bwd: negative stride");
   int64_t need = 0;
   if (int e = rvit_ssm_conv_bwd_workspace(&need, B, T, C, K)) return e;
   RVIT_CHECK_ARG(dy && dx && dw && workspace && at(workspace, 16) && workspace_bytes >= need, "ssm_conv_bwd: null pointer, or workspace of %lld bytes, %lld needed",
