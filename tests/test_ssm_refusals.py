@@ -116,3 +116,35 @@ def test_negative_strides_of_the_gradient_and_of_a_convolution():
         step[i] = -1
         assert lib.rvit_ssm_scan_step(*step, 1, 1, 1, 64, 1, 64, None) == -1 and b"stride" in lib.rvit_last_error(), i
     assert lib.rvit_ssm_conv_step(64, -1, 64, None, 64, 64, 1, 1, 8, 4, 0, None) == -1 and b"stride" in lib.rvit_last_error()
+
+
+def test_sizes_no_launch_can_take_are_refused():
+    """A launch has fewer than 2^32 threads: what would need more is refused by size (no kernel, no launch error), for a training
+    call before its forward pass."""
+    from vit_amd import _lib
+    lib = _lib.load()
+    n = ctypes.c_int64(0)
+    text = lambda: lib.rvit_last_error()  # noqa: E731
+    # scan, backward: 512 threads for each (sample, chunk, group)
+    assert lib.rvit_ssm_scan_plan(ctypes.byref(n), None, None, 1 << 22, 128, 1, 64, 1, 16) == 0
+    assert lib.rvit_ssm_scan_plan(None, None, ctypes.byref(n), 1 << 22, 128, 1, 64, 1, 16) == -1 and b"backward" in text()
+    assert lib.rvit_ssm_scan_plan(None, None, ctypes.byref(n), (1 << 22) - 1, 128, 1, 64, 1, 16) == 0
+    assert lib.rvit_ssm_scan_plan(None, None, ctypes.byref(n), 1, 64, (1 << 24) - 1, 1, 1, 1) == -1
+    # a sample's heads of more channels than an index over a chunk of them holds
+    assert lib.rvit_ssm_scan_plan(ctypes.byref(n), None, None, 1, 64, 1, 1 << 24, 1, 16) == -1 and b"channels" in text()
+    # convolution: backward 256 threads for each (sample, 8 strips, 32 accesses), its sums, forward
+    assert lib.rvit_ssm_conv_bwd_workspace(ctypes.byref(n), 1 << 24, 1, 4, 4) == -1 and b"ssm_conv" in text()
+    assert lib.rvit_ssm_conv_bwd_workspace(ctypes.byref(n), (1 << 24) - 1, 1, 4, 4) == 0
+    assert lib.rvit_ssm_conv_bwd_workspace(ctypes.byref(n), 1, 1, 1 << 28, 4) == -1 and b"ssm_conv" in text()
+    bwd = lambda B, C: lib.rvit_ssm_conv_bwd(64, C, C, 64, None, None, None, 64, C, C, None, 64, 64, None, None, 64, 1 << 50, 1, B, 1, C, 4, 0, None)  # noqa: E731
+    assert bwd(1 << 24, 4) == -1 and b"ssm_conv" in text()
+    assert bwd((1 << 24) - 1, 33) == -1 and b"ssm_conv" in text()       # two blocks of one-channel accesses
+    assert lib.rvit_ssm_conv_fwd(64, 1, 1, 64, None, None, None, 64, None, 1, 1 << 12, (1 << 28) - 1, 17, 4, 0, None) == -1 and b"ssm_conv" in text()
+    # norms: 64 threads a row, 256 where a row takes a workgroup; backward 256 a part, and a sample with its own gate is one at least
+    fwd = lambda rows, E: lib.rvit_sandwich_norm_fwd(64, 1, 64, 1, None, 0, 1, 1.0, 64, None, 64, None, 1e-5, 0, 64, 64, None, rows, 1, E, None)  # noqa: E731
+    assert fwd(1 << 26, 8) == -1 and b"sandwich" in text()
+    assert fwd(1 << 24, 2048) == -1 and b"sandwich" in text()
+    assert fwd(1 << 24, 257) == -1 and b"sandwich" in text()
+    assert lib.rvit_sandwich_norm_bwd_workspace(ctypes.byref(n), 1 << 25, 2, 8, 2) == -1 and b"sandwich" in text()
+    assert lib.rvit_sandwich_norm_bwd_workspace(ctypes.byref(n), (1 << 25) - 2, 2, 8, 2) == 0
+    assert lib.rvit_sandwich_norm_bwd_workspace(ctypes.byref(n), 1 << 30, 2, 8, 1) == 0

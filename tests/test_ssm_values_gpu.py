@@ -181,3 +181,23 @@ def test_fp32_decays_keep_their_low_bits(dev):
     ssm.selective_scan_step(zero[:, 0], 20 * dt[:, 0].to(dev), A.to(dev), one[:, 0], one[:, 0], st)
     want = torch.exp((20 * dt[:, 0]).double() * A.double())
     _within("step", st[..., 0, 0], want, 2.0 ** -22 * want)
+
+
+def test_sizes_no_launch_can_take(dev):
+    """More threads than a launch has: ValueError, a training call's before anything ran."""
+    from vit_amd import ssm
+    e = torch.ones(1, device=dev)
+    big = torch.zeros(2 ** 26, 1, device=dev, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="sandwich_norm"):
+        ssm.sandwich_norm(big, big, e, None, e, None)
+    x, w = big[:2 ** 24].unsqueeze(1), torch.ones(1, 2, device=dev, requires_grad=True)
+    with pytest.raises(ValueError, match="ssm_conv"):
+        ssm.causal_conv(x, w)
+    assert ssm.causal_conv(x, w.detach()).shape == x.shape
+    pair = big[:2 ** 25].view(2 ** 24, 2, 1)
+    with pytest.raises(ValueError, match="sandwich_norm"):
+        ssm.sandwich_norm(pair, pair, e.clone().requires_grad_(), None, e, None, gate=big[:2 ** 24])
+    one = torch.zeros(2 ** 23, 1, 1, 1, device=dev, dtype=torch.bfloat16)
+    a = torch.full((1,), -1.0, device=dev, requires_grad=True)
+    with pytest.raises(ValueError, match="backward"):
+        ssm.selective_scan(one, one[..., 0], a, one, one)

@@ -45,6 +45,10 @@ void split_heads(SsmBwdArgs& a) {
   a.hsplit = (r + a.hper - 1) / a.hper;
 }
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
+// (a launch has fewer than 2^32 threads; the chunk kernel has 512 a workgroup, the sums' 256)
+bool bwd_fits(const SsmBwdArgs& a) {
+  return (int64_t)a.f.B * a.f.nchunks * a.f.G * a.hsplit < (1 << 23) && a.f.H < (1 << 23);
+}
 
 int shape(SsmScanArgs& a, int dtype, int B, int T, int H, int P, int G, int N) {
   RVIT_CHECK_ARG(dtype == RVIT_BF16 || dtype == RVIT_F32, "ssm_scan: dtype %d", dtype);
@@ -52,6 +56,7 @@ int shape(SsmScanArgs& a, int dtype, int B, int T, int H, int P, int G, int N) {
   RVIT_CHECK_ARG(N > 0 && N <= SSM_MAX_N, "ssm_scan: %d states per channel (1 .. %d)", N, SSM_MAX_N);
   RVIT_CHECK_ARG((int64_t)B * H * ((P + 63) / 64) < (1 << 24) && (int64_t)B * ((T + 63) / 64) * H < (1 << 30) && T < (1 << 28),
                  "ssm_scan: too many rows");
+  RVIT_CHECK_ARG(P < (1 << 24), "ssm_scan: %d channels a head (under 2^24)", P);
   a.B = B; a.T = T; a.H = H; a.P = P; a.G = G; a.N = N;
   segments(a);
   return RVIT_OK;
@@ -87,6 +92,7 @@ int rvit_ssm_scan_plan(int64_t* fwd_bytes, int64_t* state_floats, int64_t* bwd_b
   SsmBwdArgs a = {};
   if (int e = shape(a.f, RVIT_F32, B, T, H, P, G, N)) return e;
   split_heads(a);
+  RVIT_CHECK_ARG(!bwd_bytes || bwd_fits(a), "ssm_scan: more samples, chunks of 64 tokens and groups than a backward pass can take (B=%d T=%d G=%d H=%d)", B, T, G, H);
   if (fwd_bytes) *fwd_bytes = seg_bytes(a.f) + 16;
   if (state_floats) *state_floats = (int64_t)a.f.nchunks * a.f.seg_stride;
   if (bwd_bytes)
@@ -217,6 +223,9 @@ int rvit_ssm_conv_bwd_workspace(int64_t* bytes, int B, int T, int C, int K) {
   RVIT_CHECK_ARG(B > 0 && T > 0 && C > 0 && K >= 2 && K <= 6 && bytes, "ssm_conv: bad sizes B=%d T=%d C=%d K=%d (K: 2 .. 6)", B, T, C, K);
   int strip, n;
   bwd_strips(strip, n, B, T, C);
+  const int64_t blocks = (int64_t)B * ((n + 7) / 8) * (((int64_t)C + 127) / 128);      // at four channels an access
+  RVIT_CHECK_ARG(blocks < (1 << 24) && (int64_t)(K + 1) * C < (1 << 28), "ssm_conv: more samples, tokens and channels than a backward pass can take (B=%d T=%d C=%d)",
+                 B, T, C);
   *bytes = (int64_t)B * ((n + 7) / 8) * (K + 1) * C * 4;
   return RVIT_OK;
 }
@@ -302,6 +311,7 @@ int rvit_sandwich_norm_bwd_workspace(int64_t* bytes, int64_t rows, int T, int E,
   SandwichArgs a = {};
   a.rows = rows; a.T = T > 0 ? T : 1; a.E = E; a.gate_kind = gate_kind;
   sandwich_parts(a);
+  RVIT_CHECK_ARG(a.parts < (1 << 24), "sandwich_norm: %d samples with gates are more than a backward pass can take", a.parts);
   *bytes = (int64_t)a.parts * 5 * E * 4;
   return RVIT_OK;
 }

@@ -375,6 +375,7 @@ int launch_bwd(const SandwichArgs& a, hipStream_t st) {
 template <typename TR, typename TY, int V, int WPR, int IT>
 int launch_fwd(const SandwichArgs& a, hipStream_t st) {
   constexpr int R = 4 / WPR;
+  RVIT_CHECK_ARG((a.rows + R - 1) / R < (1 << 24), "sandwich_norm: %ld rows of %d columns are more than a launch can take", a.rows, a.E);
   hipLaunchKernelGGL((sandwich_fwd_kernel<TR, TY, V, WPR, IT>), dim3((unsigned)((a.rows + R - 1) / R)), dim3(256), 0, st, a);
   RVIT_CHECK_LAUNCH("sandwich_fwd");
   return RVIT_OK;

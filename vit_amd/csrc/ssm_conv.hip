@@ -295,7 +295,9 @@ int launch(const SsmConvArgs& a, int what, hipStream_t st) {
   if constexpr (V < 8) {      // (eight channels a thread: forward only, see below)
     if (what == SSM_CONV_BWD) {
       const int sblocks = (a.strips + 7) / 8;
-      hipLaunchKernelGGL((ssm_conv_bwd_kernel<T, V, K>), dim3((unsigned)((groups + 31) / 32) * (a.B * sblocks)), dim3(256), 0, st, a);
+      const long blocks = (long)((groups + 31) / 32) * a.B * sblocks;
+      RVIT_CHECK_ARG(blocks < (1 << 24), "ssm_conv: more samples, tokens and channels than a backward pass can take (B=%d T=%d C=%d)", a.B, a.T, a.C);
+      hipLaunchKernelGGL((ssm_conv_bwd_kernel<T, V, K>), dim3((unsigned)blocks), dim3(256), 0, st, a);
       RVIT_CHECK_LAUNCH("ssm_conv_bwd");
       hipLaunchKernelGGL(ssm_conv_sum_kernel, dim3((unsigned)(((long)(K + 1) * a.C + 63) / 64)), dim3(1024), 0, st, a.part, a.dw, a.dbias, a.B * sblocks, a.C, K);
       RVIT_CHECK_LAUNCH("ssm_conv_sum");
@@ -303,6 +305,7 @@ int launch(const SsmConvArgs& a, int what, hipStream_t st) {
     }
   }
   const long n = (long)a.B * (what == SSM_CONV_FWD ? a.strips : 1) * groups;
+  RVIT_CHECK_ARG((n + 255) / 256 < (1 << 24), "ssm_conv: more samples, tokens and channels than a launch can take (B=%d T=%d C=%d)", a.B, a.T, a.C);
   const dim3 grid((unsigned)((n + 255) / 256));
   if (what == SSM_CONV_FWD) hipLaunchKernelGGL((ssm_conv_fwd_kernel<T, V, K>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((ssm_conv_step_kernel<T, V, K>), grid, dim3(256), 0, st, a);

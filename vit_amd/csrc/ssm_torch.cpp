@@ -31,7 +31,10 @@ void* stream(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStreamMasqu
 Tensor like(const Tensor& t) { return at::empty(t.sizes(), t.options()); }
 Tensor bytes(int64_t n, const Tensor& t) { return at::empty({n}, t.options().dtype(at::kByte)); }
 
-void done(int status, const char* what) { TORCH_CHECK(status == 0, what, " failed with status ", status, ": ", rvit_last_error()); }
+void done(int status, const char* what) {
+  TORCH_CHECK_VALUE(status != RVIT_EINVAL, what, ": ", rvit_last_error());
+  TORCH_CHECK(status == 0, what, " failed with status ", status, ": ", rvit_last_error());
+}
 
 void check_f32(const Tensor& t, at::IntArrayRef shape, const char* op, const char* name) {
   TORCH_CHECK_VALUE(!t.defined() || (t.scalar_type() == at::kFloat && t.sizes() == shape && t.is_contiguous()), op, ": ", name, " must be contiguous float32 ",
@@ -122,6 +125,10 @@ struct Conv : torch::autograd::Function<Conv> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Opt& bias_, bool silu, const Opt& state_, const Opt& lengths_,
                                bool want_state) {
     const Tensor bias = get(bias_), state = get(state_), lengths = get(lengths_);
+    const char* op = "causal_conv";
+    int64_t nb = 0;      // (what the backward pass cannot take is refused here)
+    if (x.size(1))
+      done(rvit_ssm_conv_bwd_workspace(&nb, size(x.size(0), op), size(x.size(1), op), size(x.size(2), op), (int)w.size(1)), "rvit_ssm_conv_bwd_workspace");
     auto out = conv_run(x, w, bias, silu, state, lengths, want_state);
     ctx->save_for_backward({x, w, bias, state, lengths});
     ctx->saved_data["silu"] = silu;
@@ -218,8 +225,8 @@ ScanOut scan_run(const Tensor& x, const Tensor& dt, const Tensor& A, const Tenso
                  const Tensor& state, const Tensor& lengths, bool want_state, bool train) {
   const c10::DeviceGuard guard(x.device());
   const Dims d(x, Bm, false);
-  int64_t fwd = 0, floats = 0;
-  done(rvit_ssm_scan_plan(&fwd, &floats, nullptr, d.B, d.T, d.H, d.P, d.G, d.N), "rvit_ssm_scan_plan");
+  int64_t fwd = 0, floats = 0, bwd = 0;
+  done(rvit_ssm_scan_plan(&fwd, &floats, train ? &bwd : nullptr, d.B, d.T, d.H, d.P, d.G, d.N), "rvit_ssm_scan_plan");
   ScanOut o;
   o.y = like(x);
   if (want_state) o.after = at::empty({d.B, d.H, d.P, d.N}, A.options());
@@ -356,7 +363,11 @@ struct Sandwich : torch::autograd::Function<Sandwich> {
   static variable_list forward(AutogradContext* ctx, const Tensor& residual, const Tensor& y, const Tensor& pw, const Opt& pb_, const Tensor& nw, const Opt& nb_,
                                const Opt& gate_, int64_t kind, double scale, bool rms, double eps) {
     const Tensor pb = get(pb_), nb = get(nb_), gate = get(gate_);
-    const Tensor stats = at::empty({y.numel() / y.size(-1), 4}, pw.options());
+    const int64_t rows = y.numel() / y.size(-1);
+    int64_t nbytes = 0;      // (what the backward pass cannot take is refused here)
+    if (rows)
+      done(rvit_sandwich_norm_bwd_workspace(&nbytes, rows, size(y.size(-2), "sandwich_norm"), (int)y.size(-1), (int)kind), "rvit_sandwich_norm_bwd_workspace");
+    const Tensor stats = at::empty({rows, 4}, pw.options());
     const auto out = sandwich_run(residual, y, pw, pb, nw, nb, gate, (int)kind, scale, rms, eps, stats);
     ctx->save_for_backward({residual, y, pw, pb, nw, nb, gate, stats});
     ctx->saved_data["kind"] = kind;
