@@ -148,3 +148,9 @@ def test_sizes_no_launch_can_take_are_refused():
     assert lib.rvit_sandwich_norm_bwd_workspace(ctypes.byref(n), 1 << 25, 2, 8, 2) == -1 and b"sandwich" in text()
     assert lib.rvit_sandwich_norm_bwd_workspace(ctypes.byref(n), (1 << 25) - 2, 2, 8, 2) == 0
     assert lib.rvit_sandwich_norm_bwd_workspace(ctypes.byref(n), 1 << 30, 2, 8, 1) == 0
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_an_empty_batch_is_no_error_of_shape(name):
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        _calls(batch=0)[name]()

@@ -201,3 +201,29 @@ def test_sizes_no_launch_can_take(dev):
     a = torch.full((1,), -1.0, device=dev, requires_grad=True)
     with pytest.raises(ValueError, match="backward"):
         ssm.selective_scan(one, one[..., 0], a, one, one)
+
+
+def test_empty_batch(dev):
+    """No samples: empty results, untouched states, gradients of zero; as the norms have it."""
+    from vit_amd import ssm
+    for T in (0, 5):
+        s = to(scan_inputs(90, torch.bfloat16, 2, 5, 4, 8, 2, 16, state=True), dev)
+        s = {k: v[:0, :T] if k in ("x", "dt", "Bm", "Cm", "z") else v[:0] if k == "state" else v for k, v in s.items()}
+        lens = torch.zeros(0, dtype=torch.int32, device=dev)
+        y, end = _call(ssm, s, lengths=lens, return_state=True)
+        assert y.shape == (0, T, 4, 8) and end.shape == (0, 4, 8, 16)
+        leaf = {k: v.detach().requires_grad_() for k, v in s.items()}
+        y, end = _call(ssm, leaf, return_state=True)
+        for k, g in zip(leaf, torch.autograd.grad([y, end], list(leaf.values()), [torch.zeros_like(y), torch.zeros_like(end)])):
+            assert g.shape == leaf[k].shape and not bool(g.count_nonzero()), k
+        x, w, st = torch.zeros(0, T, 8, device=dev), torch.ones(8, 4, device=dev), torch.zeros(0, 3, 8, device=dev)
+        y, end = ssm.causal_conv(x, w, state=st, lengths=lens, return_state=True)
+        assert y.shape == (0, T, 8) and end.shape == (0, 3, 8)
+        w.requires_grad_()
+        (dw,) = torch.autograd.grad(ssm.causal_conv(x, w, activation="silu").sum(), [w])
+        assert not bool(dw.count_nonzero())
+    y = ssm.selective_scan_step(s["x"].new_zeros(0, 4, 8), s["dt"].new_zeros(0, 4), s["A"], s["Bm"].new_zeros(0, 2, 16), s["Cm"].new_zeros(0, 2, 16), s["state"])
+    assert y.shape == (0, 4, 8)
+    assert ssm.causal_conv_step(torch.zeros(0, 8, device=dev), torch.ones(8, 4, device=dev), None, st).shape == (0, 8)
+    e = torch.ones(8, device=dev)
+    assert ssm.sandwich_norm(torch.zeros(0, 3, 8, device=dev), torch.zeros(0, 3, 8, device=dev), e, None, e, None)[1].shape == (0, 3, 8)

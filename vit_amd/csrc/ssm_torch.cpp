@@ -100,7 +100,7 @@ Opt some(const Tensor& t) { return t.defined() ? Opt(t) : Opt(); }
 void conv_shapes(const char* op, const Tensor& x, const Tensor& w, const Tensor& bias, bool step) {
   TORCH_CHECK_VALUE(x.dim() == (step ? 2 : 3) && any_type(x), op, ": x must be bf16 / f32 ", step ? "[B,C]" : "[B,T,C]", ", got ", x.scalar_type(), " ", x.sizes());
   const int64_t C = x.size(-1);
-  TORCH_CHECK_VALUE(w.dim() == 2 && w.size(0) == C && w.size(1) >= 2 && w.size(1) <= 6 && x.size(0) >= 1 && C >= 1, op, ": weight must be [C=", C, ", 2..6], got ",
+  TORCH_CHECK_VALUE(w.dim() == 2 && w.size(0) == C && w.size(1) >= 2 && w.size(1) <= 6 && C >= 1, op, ": weight must be [C=", C, ", 2..6], got ",
                     w.sizes());
   check_f32(w, w.sizes(), op, "weight");
   check_f32(bias, {C}, op, "bias");
@@ -111,7 +111,7 @@ std::pair<Tensor, Tensor> conv_run(const Tensor& x, const Tensor& w, const Tenso
   const int64_t B = x.size(0), T = x.size(1), C = x.size(2), K = w.size(1);
   Tensor y = like(x), after;
   if (want_state) after = at::empty({B, K - 1, C}, x.options());
-  if (T == 0) {      // no tokens: nothing runs, the kept inputs stay
+  if (B == 0 || T == 0) {      // no tokens: nothing runs, the kept inputs stay
     if (want_state) state.defined() ? after.copy_(state) : after.zero_();
     return {y, after};
   }
@@ -127,7 +127,7 @@ struct Conv : torch::autograd::Function<Conv> {
     const Tensor bias = get(bias_), state = get(state_), lengths = get(lengths_);
     const char* op = "causal_conv";
     int64_t nb = 0;      // (what the backward pass cannot take is refused here)
-    if (x.size(1))
+    if (x.numel())
       done(rvit_ssm_conv_bwd_workspace(&nb, size(x.size(0), op), size(x.size(1), op), size(x.size(2), op), (int)w.size(1)), "rvit_ssm_conv_bwd_workspace");
     auto out = conv_run(x, w, bias, silu, state, lengths, want_state);
     ctx->save_for_backward({x, w, bias, state, lengths});
@@ -144,7 +144,7 @@ struct Conv : torch::autograd::Function<Conv> {
     const int64_t B = x.size(0), T = x.size(1), C = x.size(2), K = w.size(1);
     Tensor dx = like(x), dw = like(w), db = bias.defined() ? like(bias) : Tensor(), ds = state.defined() ? like(state) : Tensor();
     const Tensor dafter = g.size() > 1 ? dense(g[1]) : Tensor();
-    if (T == 0) {
+    if (B == 0 || T == 0) {
       dw.zero_();
       if (db.defined()) db.zero_();
       if (ds.defined()) dafter.defined() ? ds.copy_(dafter) : ds.zero_();
@@ -186,6 +186,7 @@ Tensor conv_step(Tensor x, const Tensor& w, const Opt& bias_, const Tensor& stat
   const c10::DeviceGuard guard(x.device());
   x = packed(x, 1);
   const Tensor y = like(x);
+  if (x.size(0) == 0) return y;
   done(rvit_ssm_conv_step(ptr(x), x.stride(0), w.data_ptr<float>(), (const float*)ptr(bias), ptr(state), ptr(y), dtype(x), size(x.size(0), "causal_conv_step"),
                           size(x.size(1), "causal_conv_step"), (int)w.size(1), silu, stream(x)),
        "rvit_ssm_conv_step");
@@ -208,7 +209,7 @@ void scan_shapes(const char* op, const Tensor& x, const Tensor& dt, const Tensor
   TORCH_CHECK_VALUE(Bm.dim() == lead + 2 && Bm.sizes() == Cm.sizes() && Bm.sizes().slice(0, lead) == x.sizes().slice(0, lead), op, ": Bm and Cm must be ",
                     step ? "[B,G,N]" : "[B,T,G,N]", ", got ", Bm.sizes(), " and ", Cm.sizes());
   const int64_t H = x.size(-2), P = x.size(-1), G = Bm.size(-2), N = Bm.size(-1);
-  TORCH_CHECK_VALUE(x.size(0) >= 1 && H >= 1 && P >= 1 && G >= 1 && N >= 1 && H % G == 0 && N <= 128, op, ": ", H, " heads in ", G, " groups, ", P, " channels, ", N,
+  TORCH_CHECK_VALUE(H >= 1 && P >= 1 && G >= 1 && N >= 1 && H % G == 0 && N <= 128, op, ": ", H, " heads in ", G, " groups, ", P, " channels, ", N,
                     " states (at most 128)");
   TORCH_CHECK_VALUE(dt.sizes() == x.sizes().slice(0, lead + 1), op, ": dt must be ", x.sizes().slice(0, lead + 1), ", got ", dt.sizes());
   TORCH_CHECK_VALUE(!z.defined() || z.sizes() == x.sizes(), op, ": z must be ", x.sizes(), ", got ", z.sizes());
@@ -224,11 +225,15 @@ struct ScanOut { Tensor y, after, v, states; };
 ScanOut scan_run(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& Bm, const Tensor& Cm, const Tensor& D, const Tensor& z, const Tensor& dt_bias,
                  const Tensor& state, const Tensor& lengths, bool want_state, bool train) {
   const c10::DeviceGuard guard(x.device());
+  ScanOut o;
+  o.y = like(x);
+  if (x.size(0) == 0) {      // no samples: nothing runs
+    if (want_state) o.after = at::empty({0, x.size(2), x.size(3), Bm.size(3)}, A.options());
+    return o;
+  }
   const Dims d(x, Bm, false);
   int64_t fwd = 0, floats = 0, bwd = 0;
   done(rvit_ssm_scan_plan(&fwd, &floats, train ? &bwd : nullptr, d.B, d.T, d.H, d.P, d.G, d.N), "rvit_ssm_scan_plan");
-  ScanOut o;
-  o.y = like(x);
   if (want_state) o.after = at::empty({d.B, d.H, d.P, d.N}, A.options());
   if (train && z.defined()) o.v = at::empty(x.sizes(), A.options());
   if (train) o.states = at::empty({floats}, A.options());
@@ -262,7 +267,7 @@ struct Scan : torch::autograd::Function<Scan> {
     Tensor dz = z.defined() ? like(x) : Tensor(), dD = D.defined() ? like(D) : Tensor(), dbias = dt_bias.defined() ? like(dt_bias) : Tensor();
     Tensor ds = ctx->saved_data["state"].toBool() ? at::empty({d.B, d.H, d.P, d.N}, A.options()) : Tensor();
     const Tensor dafter = g.size() > 1 ? dense(g[1]) : Tensor();
-    if (d.T == 0) {
+    if (d.B == 0 || d.T == 0) {
       for (const Tensor& t : {dA, dD, dbias})
         if (t.defined()) t.zero_();
       if (ds.defined()) dafter.defined() ? ds.copy_(dafter) : ds.zero_();
@@ -318,6 +323,7 @@ Tensor scan_step(Tensor x, Tensor dt, const Tensor& A, Tensor Bm, Tensor Cm, con
   z = packed(z, 2);
   const Dims d(x, Bm, true);
   const Tensor y = like(x);
+  if (d.B == 0) return y;
   done(rvit_ssm_scan_step(ptr(x), x.stride(0), ptr(dt), dt.stride(0), A.data_ptr<float>(), ptr(Bm), Bm.stride(0), ptr(Cm), Cm.stride(0), (const float*)ptr(D), ptr(z),
                           stride(z, 0), (const float*)ptr(dt_bias), (float*)ptr(state), ptr(y), dtype(x), d.B, d.H, d.P, d.G, d.N, stream(x)),
        "rvit_ssm_scan_step");

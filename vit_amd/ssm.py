@@ -2,12 +2,13 @@
 token at a time) and the norms around a block, on librvit (csrc/ssm_conv.hip, ssm_scan.hip, ssm_scan_bwd.hip, sandwich.hip)
 through the torch binding csrc/ssm_torch.cpp.  The temporal encoder's `model_type='ssm'` (vit_amd/sequence.py) is built of them.
 
-Tensors live on one GPU; launches go to the current stream of that GPU.  Activations are bf16 or fp32, per-channel and
-per-head parameters and kept scan states fp32.  Sums, states and statistics are fp32 or wider whatever the inputs.  Results do
+Tensors live on one GPU; launches go to the current stream of that GPU.  Activations are bf16 or fp32, per-channel and per-
+head parameters and kept scan states fp32.  Sums, states and statistics are fp32 or wider whatever the inputs.  Results do
 not depend on the order in which workgroups run.  First derivatives in reverse mode only: dual tensors (forward mode) and
-create_graph=True raise RuntimeError, as does torch.jit.trace.  Wrong shapes, types and devices raise ValueError, a CPU tensor
-RuntimeError: there is no CPU path.  Calls can be captured into graphs, training steps with their backward passes too (these
-only while no eager autograd graph of the same leaves is alive, as for every torch operation)."""
+create_graph=True raise RuntimeError, as does torch.jit.trace.  Wrong shapes, types and devices raise ValueError, a CPU
+tensor RuntimeError: there is no CPU path.  An empty batch, or no tokens, gives empty results and leaves states as they are.
+Calls can be captured into graphs, training steps with their backward passes too (these only while no eager autograd graph of
+the same leaves is alive, as for every torch operation)."""
 from __future__ import annotations
 
 import os
