@@ -227,3 +227,37 @@ def test_empty_batch(dev):
     assert ssm.causal_conv_step(torch.zeros(0, 8, device=dev), torch.ones(8, 4, device=dev), None, st).shape == (0, 8)
     e = torch.ones(8, device=dev)
     assert ssm.sandwich_norm(torch.zeros(0, 3, 8, device=dev), torch.zeros(0, 3, 8, device=dev), e, None, e, None)[1].shape == (0, 3, 8)
+
+
+def test_what_stands_behind_a_samples_last_frame_does_not_count(dev):
+    """A padded batch through the encoder: NaN behind the ends gives the features and gradients of any other padding, bit for bit
+    (with the ordered reductions: the first norm's weight gradient is a sum of atomics without); a sample of no frames too."""
+    from vit_amd import ops
+    from vit_amd.sequence import TemporalEncoder
+    torch.manual_seed(3)
+    enc = TemporalEncoder(128, 64, 2, dropout=0.0, bidirectional=False, model_type="ssm").to(dev).train()
+    lens = torch.tensor([9, 1, 4, 0], dtype=torch.int32, device=dev)
+    x = torch.randn(4, 9, 128, device=dev)
+    behind = torch.arange(9, device=dev)[None] >= lens[:, None]
+    cot = torch.randn(4, 64, device=dev)
+
+    def run(fill):
+        xs = x.masked_fill(behind[..., None], fill).requires_grad_()
+        got, _ = enc.ssm_features(xs, lens)
+        return [got.detach()] + list(torch.autograd.grad(got, [p for _, p in enc.named_parameters()] + [xs], cot))
+
+    was = ops.ordered_reductions_enabled(dev)
+    ops.enable_ordered_reductions(dev)
+    try:
+        want = run(0.0)
+        assert all(bool(torch.isfinite(v).all()) for v in want) and float(want[-1][behind].abs().max()) == 0.0
+        for fill in (float("nan"), float("inf"), 3.0):
+            for a, b in zip(run(fill), want):
+                assert torch.equal(a, b), fill
+    finally:
+        ops.enable_ordered_reductions(dev, was)
+    with torch.no_grad():
+        assert float(enc.ssm_features(x, lens)[0][3].abs().max()) == 0.0      # no frame, no feature
+    for bad in (lens.long(), lens[:3], lens.cpu()):
+        with pytest.raises(ValueError, match="lengths"):
+            enc.ssm_features(x, bad)

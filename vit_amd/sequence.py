@@ -265,20 +265,26 @@ class TemporalEncoder(nn.Module):
         return _TemporalFunction.apply(x, self, None, self.training and torch.is_grad_enabled(), *self.parameters())
 
     def ssm_features(self, x: torch.Tensor, lengths: Optional[torch.Tensor] = None, cache: Optional[list] = None):
-        """-> (feature [B,hidden] fp32 of each sample's last frame, seed of this pass's dropout sites)."""
+        """-> (feature [B,hidden] fp32 of each sample's last frame, seed of this pass's dropout sites).  `lengths` int32 [B]: sample b
+        ends after lengths[b] frames (held to 0..T), and what x holds behind counts nowhere; without a frame its feature is zero."""
         if not x.is_cuda:
             raise RuntimeError("the temporal encoder runs on the GPU through librvit only; there is no CPU fallback")
         if x.dim() != 3 or x.shape[2] != self.rnn.input_size or x.shape[0] < 1 or x.shape[1] < 1:
             raise ValueError(f"expected features [B,T,{self.rnn.input_size}], got {tuple(x.shape)}")
+        if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != x.shape[:1] or lengths.device != x.device):
+            raise ValueError(f"lengths must be int32 [{x.shape[0]}] on {x.device}, got {lengths.dtype} {tuple(lengths.shape)} on {lengths.device}")
         train = self.training and torch.is_grad_enabled()
         base = int(torch.randint(0, 2 ** 62, (1,)).item()) if train else 0
         with torch.cuda.device(x.device):
+            if lengths is not None:      # zero, not only unread: the weights' gradients are products with every row
+                ends = lengths.long().clamp(0, x.shape[1])[:, None]
+                x = torch.where((torch.arange(x.shape[1], device=x.device) < ends)[..., None], x, x.new_zeros(()))
             n = self.rnn.run(x, lengths, self.dropout if train else 0.0, base, cache)
             if lengths is None:
                 last = n[:, -1]
             else:
-                at = (lengths.long().clamp(1, x.shape[1]) - 1)[:, None, None].expand(-1, 1, n.shape[2])
-                last = n.gather(1, at)[:, 0]
+                last = n.gather(1, (ends - 1).clamp(min=0)[..., None].expand(-1, 1, n.shape[2]))[:, 0]
+                last = torch.where(ends > 0, last, last.new_zeros(()))
             return last.float(), base
 
 
