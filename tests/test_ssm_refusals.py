@@ -154,3 +154,14 @@ def test_sizes_no_launch_can_take_are_refused():
 def test_an_empty_batch_is_no_error_of_shape(name):
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         _calls(batch=0)[name]()
+
+
+def test_a_learned_scale_is_refused():
+    """A tensor would be read as a number, its gradient lost: a learned scale belongs into the gate."""
+    from vit_amd import ssm
+    x, e = torch.ones(2, 8), torch.ones(8)
+    for scale in (torch.ones((), requires_grad=True), torch.nn.Parameter(torch.ones(1)), torch.ones(())):
+        with pytest.raises(ValueError, match="scale"):
+            ssm.sandwich_norm(x, x, e, None, e, None, scale=scale)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ssm.sandwich_norm(x, x, e, None, e, None, scale=2)

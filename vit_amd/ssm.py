@@ -110,6 +110,8 @@ def sandwich_norm(residual: torch.Tensor, y: torch.Tensor, post_weight: torch.Te
     [B,T,E]: one per sample) or like y, fp32 or y's dtype; scale a number."""
     if kind not in ("layer", "rms"):
         raise ValueError(f"sandwich_norm: kind {kind!r} ('layer' or 'rms')")
+    if isinstance(scale, torch.Tensor):
+        raise ValueError("sandwich_norm: scale must be a number (a tensor's gradient would be lost: a learned scale belongs into the gate)")
     rms = kind == "rms"
     if rms and (post_bias is not None or pre_bias is not None):
         raise ValueError("sandwich_norm: kind 'rms' has no biases")
