@@ -261,3 +261,46 @@ def test_what_stands_behind_a_samples_last_frame_does_not_count(dev):
     for bad in (lens.long(), lens[:3], lens.cpu()):
         with pytest.raises(ValueError, match="lengths"):
             enc.ssm_features(x, bad)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("T", [1, 8, 63, 64])
+@pytest.mark.parametrize("P,N", [(24, 16), (64, 64), (100, 100), (64, 128), (24, 128), (100, 64)])
+def test_one_chunk_without_a_state(dev, P, N, T, dtype):
+    """The backward pass of one chunk where no gradient of a state comes in or goes out: nothing is swept."""
+    from vit_amd import ssm
+    s = scan_inputs(T + P + N, DTYPES[dtype], 2, T, 4, P, 2, N)
+    leaf = leaves64(s)
+    wy, _ = ref.selective_scan(**leaf)
+    names = [k for k in s if s[k] is not None]
+    dy = randn(torch.Generator().manual_seed(T), *wy.shape, dtype=DTYPES[dtype])
+    want = torch.autograd.grad(wy, [leaf[k] for k in names], dy.double())
+    d = {k: v if v is None else v.requires_grad_() for k, v in to(s, dev).items()}
+    y = _call(ssm, d)
+    close("y", y, wy)
+    for k, a, b in zip(names, torch.autograd.grad(y, [d[k] for k in names], dy.to(dev)), want):
+        if T == 1 and k == "A":      # one token: nothing passes through a decay
+            assert float(a.abs().max()) == 0.0
+            continue
+        close("d" + k, a, b)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("B,H", [(19, 9), (16, 16), (257, 1), (20, 15), (73, 7), (16, 32)])
+def test_row_counts_around_the_segments(dev, B, H, dtype):
+    """171 to 256 rows of eight chunks are cut in two, 257 and more are one walk: both sides of each step."""
+    from vit_amd import ssm
+    T, P, N = 513, 4, 4
+    s = scan_inputs(B + H, DTYPES[dtype], B, T, H, P, 1, N, state=True)
+    leaf = leaves64(s)
+    wy, wend = ref.selective_scan(**leaf)
+    names = [k for k in s if s[k] is not None]
+    g = torch.Generator().manual_seed(B)
+    dy, dend = randn(g, *wy.shape, dtype=DTYPES[dtype]), randn(g, *wend.shape)
+    want = torch.autograd.grad([wy, wend], [leaf[k] for k in names], [dy.double(), dend.double()])
+    d = {k: v.requires_grad_() for k, v in to(s, dev).items()}
+    y, end = _call(ssm, d, return_state=True)
+    close("y", y, wy)
+    close("end", end, wend)
+    for k, a, b in zip(names, torch.autograd.grad([y, end], [d[k] for k in names], [dy.to(dev), dend.to(dev)]), want):
+        close("d" + k, a, b)
