@@ -664,7 +664,8 @@ int rvit_ssm_conv_step(const void* x, int64_t sxb, const float* w, const float* 
  * behind the last token of each sample.  Training passes v (fp32, [B,T,H,P]; only with z) and states (fp32, state_floats of
  * rvit_ssm_scan_plan), both read by bwd.  Workspaces: fwd_bytes / bwd_bytes of rvit_ssm_scan_plan, 16-byte aligned.  bwd:
  * dA, dD, ddt_bias fp32 [H] (the last two may be null), dstate0 may be null, dz with z only.  Results do not depend on the
- * order in which workgroups run.  A non-finite input of a valid token may reach every output of its chunk of 64 tokens.
+ * order in which workgroups run.  A non-finite input of a valid token may reach every output of its chunk of 64 tokens.  A is read
+ * whatever T is.  Sizes whose launches would need 2^32 threads are RVIT_EINVAL, in rvit_ssm_scan_plan (bwd_bytes) already.
  * step: one token, x [B,H,P], state advances in place. */
 int rvit_ssm_scan_plan(int64_t* fwd_bytes, int64_t* state_floats, int64_t* bwd_bytes, int B, int T, int H, int P, int G,
                        int N);

@@ -4,7 +4,7 @@
 // registers: two rows in, two rows out.  Backward, with the rows' means and 1/std kept by the forward and h recomputed:
 //   dh' = dh + norm_pre'(dn);  du = scale gate dh';  dresidual = dh';  dgate = scale u dh';  dy = norm_post'(du)
 // Both passes are HBM bound: at 25216 x 1024, bf16 blocks in an fp32 stream, forward 64 us (4.8 TB/s), backward 101 us (4.6 TB/s) and
-// 9 us for the sums over its 1024 parts.  Forward: a wave holds a row of up to 1024 columns, a workgroup of four waves a longer one.
+// 9 us for the sums over its 1024 parts; all fp32 77 us (5.4 TB/s) and 136 us (4.6 TB/s).  Forward: a wave holds a row of up to 1024 columns, a workgroup of four waves a longer one.
 #include "ssm_common.h"
 #include "rvit_internal.h"
 #include "ssm_args.h"

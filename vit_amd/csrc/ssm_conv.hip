@@ -2,8 +2,9 @@
 // backward and the single-token form:   u[t] = bias + sum_k w[k] x[t - K + 1 + k],  y = u or silu(u).
 // HBM bound: a thread owns V channels (one 16-byte access) of a strip of tokens and slides its window through registers, so
 // x is read once but for K - 1 tokens between strips (which the caches hold), and a wave reads 1 KB of a token's row.
-// At 8 x 2048 x 1792 bf16: forward 29 us (4.0 TB/s), backward 52 us (3.4 TB/s: u is recomputed, and windows and sums of 4 channels
-// leave four waves a SIMD; more tokens on their way change nothing), the parts' sum 4 us.
+// At 8 x 2048 x 1792: forward 29 us in bf16 (4.0 TB/s), 45 in fp32 (5.2 TB/s); backward 52 us in bf16 (3.4 TB/s) and 80 in fp32 (4.4
+// TB/s), the parts' sum 4 us.  The bf16 backward pass is bound by its vector instructions: u again, silu', the window's products and
+// the tests of a strip's ends keep the SIMDs busy for 80 % of it (four waves each; more tokens on their way change nothing).
 #include "ssm_common.h"
 #include "rvit_internal.h"
 #include "ssm_args.h"

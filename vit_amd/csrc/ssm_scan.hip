@@ -69,12 +69,12 @@ __device__ __forceinline__ void scores(const T* Bs, const T* Cs, T* Gs, const fl
 // A chunk's images and decays are fetched and worked out while the chunk before it is computed.
 // YOUT = false: only the state a segment (but the last) reaches from zero, and the segment's summed log decay (long sequences of few
 // rows are cut into segments, joined by ssm_join_kernel).  VEC: all wide accesses are aligned and whole.
-// Measured, bf16, 128 states: 32768 tokens x 16 heads x 64 (segments of 16 chunks) 112 us, the pass for states 44 us;
-// [8, 2048, 24, 64] with a state kept per chunk (0.4 GB) 157 us and 39 us.  Bound by two waves a SIMD (256 registers, 69 KB of LDS):
-// vector instructions (splits, decays, the gate) fill a fifth to a quarter of a wave's time, matrix instructions a tenth, waits for
-// LDS, barriers and memory the rest.  A second x image with two barriers a chunk, and one barrier in the pass for states,
-// took the same time, as did the score tiles spread evenly over the waves; the decays are worked out by the wave with the fewest of
-// them (by wave 0 of every workgroup: 120 and 161 us).
+// Measured, bf16, 128 states: 32768 tokens x 16 heads x 64 (segments of 16 chunks) 111 us, the pass for states 45 us;
+// [8, 2048, 24, 64] with a state kept per chunk and v in 32 bits (0.45 GB) 165 us and 40 us.  Bound by two waves a SIMD (256
+// registers, 69 KB of LDS): of a wave's time vector instructions (splits, decays, the gate) fill 27 and 20 %, matrix instructions 13
+// and 9 %; waits for LDS, barriers and memory 37 and 47 %, waits for the SIMD's other wave 23 %.  A second x image with two barriers a
+// chunk, and one barrier in the pass for states, took the same time, as did the score tiles spread evenly over the waves; the decays
+// are worked out by the wave with the fewest of them (by wave 0 of every workgroup: 8 and 4 us more).
 template <typename T, int NP, bool YOUT, bool VEC>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_scan_fwd_kernel(SsmScanArgs a) {
   using O = SsmOps<T>;
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NP == 128 ? 1 : 2) void ssm_
 // Joins the segments: in place, the state a segment reached from zero becomes the state it starts from.  `reverse` runs from
 // the last segment to the first (the backward pass).  `init` [B,H,P,N] (or null) is what the first one starts from.
 // A thread takes four states of a channel through all segments, the next ones' on their way: its bytes in and out (192 rows of 2
-// segments, 25 MB: 6.2 us, with one state a thread 12.5; 16 rows of 32 segments, 34 MB: 13.6 and 14.6).
+// segments, 25 MB: 6.2 us, with one state a thread 12.5; 16 rows of 32 segments, 34 MB: 15 us either way).
 __global__ __launch_bounds__(64) void ssm_join_kernel(float* seg_state, const double* seg_decay, const float* init, long n, int P, int N, int pblocks, int NP,
                                                       long BH, int nseg, int reverse) {
   const long i = (long)blockIdx.x * 64 + threadIdx.x;      // of the four: [BH][pblocks][NP / 4][64]
@@ -339,7 +339,7 @@ __global__ __launch_bounds__(64) void ssm_join_kernel(float* seg_state, const do
 }
 
 // One token per sample: the state is read once and written once, in place; HBM bound (256 samples x 32 heads x 64 x 128, 540 MB:
-// 122 us, 4.4 TB/s, a copy of that size reaches 5.2; one sample: the launch).  A workgroup takes one (sample, head);
+// 124 us, 4.4 TB/s, a copy of that size reaches 5.2; one sample: the launch).  A workgroup takes one (sample, head);
 // LN lanes share a channel (each holds 4 states a turn), so that a wave reads whole lines of the state.
 template <typename T, int LN>
 __global__ __launch_bounds__(256) void ssm_scan_step_kernel(SsmStepArgs a) {

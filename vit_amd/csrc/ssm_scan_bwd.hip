@@ -12,8 +12,9 @@
 // da is written as a sum of what really passes through token u's decay.  The shorter form, a reverse running sum over the
 // whole sequence of dy . y - d e, takes the difference of two large equal parts at every token of a head that forgets fast,
 // and its rounding errors add up along the sequence into dA.
-// Two launches: the sweep computes dS of every chunk (from the last to the first, the gradient in registers), then every
-// chunk is on its own.
+// A sweep computes dS of every chunk (from the last to the first, the gradient in registers), then every chunk is on its own, and the
+// sums behind the chunks end it: three launches.  Sequences cut into segments take two more (the segments' ends from nothing, the
+// join); one chunk without a gradient of its end or start needs no sweep: two.
 #include "ssm_common.h"
 #include "rvit_internal.h"
 #include "ssm_args.h"
@@ -28,8 +29,8 @@ constexpr int Q = SSM_CHUNK;
 __device__ __forceinline__ float chunk_sign(int ch) { return ch & 1 ? -1.f : 1.f; }
 
 // ---- sweep: dS before a chunk = exp(L_Q) dS behind it + sum_t exp(L_t) v'_t C_t^T ----
-// One workgroup per (sample, head, 64 channels, segment), as the forward's.  At [8, 2048, 24, 64] x 128 states, bf16: 94 us for 0.3 GB
-// (3.2 TB/s; it waits for its loads and for its stores of a state per chunk), the pass for the segments' starts 51 us.
+// One workgroup per (sample, head, 64 channels, segment), as the forward's.  At [8, 2048, 24, 64] x 128 states, bf16: 96 us for 0.3 GB
+// (3.1 TB/s; it waits for its loads and for its stores of a state per chunk), the pass for the segments' starts 53 us.
 template <typename T, int NP, bool OUT, bool VEC>
 __global__ __launch_bounds__(256, 2) void ssm_scan_bwd_state_kernel(SsmBwdArgs a) {
   using O = SsmOps<T>;
@@ -187,9 +188,10 @@ __global__ __launch_bounds__(256, 2) void ssm_scan_bwd_state_kernel(SsmBwdArgs a
 // for all its heads, and the sums dB, dC over them stay in registers (wave: 16 states x 16 .. 64 tokens), so that shared
 // heads cost no atomics and no scratch where one workgroup takes them all.  A head's inputs are fetched while the head
 // before it is worked on, its states while its scores are.
-// [8, 2048, 24, 64] x 128 states, bf16: 285 - 295 us for 0.7 GB (2.5 TB/s).  Its LDS and registers allow one workgroup, two waves a
+// [8, 2048, 24, 64] x 128 states, bf16: 281 - 297 us for 0.75 GB (2.6 TB/s).  Its LDS and registers allow one workgroup, two waves a
 // SIMD: vector instructions (three-part operands, decays, sums) are a quarter of a wave's time, so half of the SIMD's, matrix
-// instructions a twelfth, LDS is busy for 40 %; the rest waits, at the head's three barriers and for LDS.  64 windows of 8 tokens, fp32: 30 us.
+// instructions a twelfth and a sixth, LDS is busy for 38 %; a wave waits for 43 % of its time, at the head's three barriers and for LDS,
+// and another 22 % for the SIMD's other wave.  64 windows of 8 tokens: fp32 31 us, bf16 22 us.
 template <typename T, int NP>
 struct BwdLds {
   using O = SsmOps<T>;

@@ -1,8 +1,8 @@
 // The state-space sequence operators as torch functions with autograd (module vit_amd._ssm, used by vit_amd/ssm.py) on the C
 // entry points of librvit.  In C++ because these operators are also called one token at a time and in training steps of short
 // windows, where the checks, allocations and argument conversions of a Python wrapper and a Python autograd node take
-// several times the kernels' time (a token's scan: 13.4 us, here 5.4, its launch alone 4; a training step of 64 windows of 8 tokens,
-// fp32: 207 us, here 107, its kernels 58).
+// several times the kernels' time (a token's scan: 13.4 us, here 5.5, its launch alone 4; a training step of 64 windows of 8 tokens,
+// fp32: 207 us, here 105, its kernels 56).
 // Nothing is kept from one call for the next.
 #include <torch/extension.h>
 
