@@ -165,3 +165,14 @@ def test_a_learned_scale_is_refused():
             ssm.sandwich_norm(x, x, e, None, e, None, scale=scale)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         ssm.sandwich_norm(x, x, e, None, e, None, scale=2)
+
+
+def test_odd_widths_no_backward_launch_can_take_are_refused_beforehand():
+    """Channels that are no multiple of four are taken one an access: their backward pass has four times the workgroups, and the
+    forward pass of a training call has to know."""
+    from vit_amd import _lib
+    lib = _lib.load()
+    n = ctypes.c_int64(0)
+    assert lib.rvit_ssm_conv_bwd_workspace(ctypes.byref(n), 1 << 23, 1, 33, 4) == -1 and b"ssm_conv" in lib.rvit_last_error()
+    assert lib.rvit_ssm_conv_bwd_workspace(ctypes.byref(n), (1 << 23) - 1, 1, 33, 4) == 0
+    assert lib.rvit_ssm_conv_bwd_workspace(ctypes.byref(n), 1 << 23, 1, 36, 4) == 0

@@ -223,7 +223,8 @@ int rvit_ssm_conv_bwd_workspace(int64_t* bytes, int B, int T, int C, int K) {
   RVIT_CHECK_ARG(B > 0 && T > 0 && C > 0 && K >= 2 && K <= 6 && bytes, "ssm_conv: bad sizes B=%d T=%d C=%d K=%d (K: 2 .. 6)", B, T, C, K);
   int strip, n;
   bwd_strips(strip, n, B, T, C);
-  const int64_t blocks = (int64_t)B * ((n + 7) / 8) * (((int64_t)C + 127) / 128);      // at four channels an access
+  const int64_t wide = C % 4 ? 32 : 128;      // channels of a workgroup: 32 accesses of one or (aligned) four
+  const int64_t blocks = (int64_t)B * ((n + 7) / 8) * ((C + wide - 1) / wide);
   RVIT_CHECK_ARG(blocks < (1 << 24) && (int64_t)(K + 1) * C < (1 << 28), "ssm_conv: more samples, tokens and channels than a backward pass can take (B=%d T=%d C=%d)",
                  B, T, C);
   *bytes = (int64_t)B * ((n + 7) / 8) * (K + 1) * C * 4;
