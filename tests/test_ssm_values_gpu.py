@@ -304,3 +304,94 @@ def test_row_counts_around_the_segments(dev, B, H, dtype):
     close("end", end, wend)
     for k, a, b in zip(names, torch.autograd.grad([y, end], [d[k] for k in names], [dy.to(dev), dend.to(dev)]), want):
         close("d" + k, a, b)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_gradients_through_one_output_only(dev, dtype):
+    """A loss on the returned states alone, or on one of the norms' two results."""
+    from vit_amd import ssm
+    dt = DTYPES[dtype]
+    for T in (5, 130):
+        s = scan_inputs(100 + T, dt, 2, T, 4, 24, 2, 20, state=True)
+        leaf = leaves64(s)
+        _, wend = ref.selective_scan(**leaf)
+        names = ("x", "dt", "A", "Bm", "dt_bias", "state")
+        dend = randn(torch.Generator().manual_seed(T), *wend.shape)
+        want = torch.autograd.grad(wend, [leaf[k] for k in names], dend.double())
+        d = {k: v.requires_grad_() for k, v in to(s, dev).items()}
+        _, end = _call(ssm, d, return_state=True)
+        for k, a, b in zip(names, torch.autograd.grad(end, [d[k] for k in names], dend.to(dev)), want):
+            close("d" + k, a, b)
+        x, w, st = randn(torch.Generator().manual_seed(1), 2, T, 8, dtype=dt), randn(torch.Generator().manual_seed(2), 8, 4), randn(torch.Generator().manual_seed(3), 2, 3, 8, dtype=dt)
+        x64, st64 = x.double().requires_grad_(), st.double().requires_grad_()
+        _, wend = ref.causal_conv(x64, w.double(), silu=True, state=st64)
+        gx, gs = x.to(dev).requires_grad_(), st.to(dev).requires_grad_()
+        _, end = ssm.causal_conv(gx, w.to(dev), activation="silu", state=gs, return_state=True)
+        cot = torch.ones_like(end)
+        for a, b in zip(torch.autograd.grad(end, [gx, gs], cot), torch.autograd.grad(wend, [x64, st64], cot.double().cpu())):
+            assert torch.equal(a.double().cpu(), b)      # inputs handed on
+    g = torch.Generator().manual_seed(110)
+    s = dict(residual=randn(g, 3, 7, 40, dtype=dt), y=randn(g, 3, 7, 40, dtype=dt), post_weight=randn(g, 40, shift=1.0), post_bias=randn(g, 40),
+             pre_weight=randn(g, 40, shift=1.0), pre_bias=randn(g, 40), gate=randn(g, 3, 40))
+    for which, names in ((0, ("residual", "y", "post_weight", "post_bias", "gate")), (1, tuple(s))):
+        leaf = leaves64(s)
+        out = ref.sandwich_norm(**leaf)[which]
+        cot = randn(g, *out.shape, dtype=dt)
+        want = torch.autograd.grad(out, [leaf[k] for k in names], cot.double())
+        d = {k: v.to(dev).requires_grad_() for k, v in s.items()}
+        got = torch.autograd.grad(ssm.sandwich_norm(**d)[which], [d[k] for k in names], cot.to(dev))
+        for k, a, b in zip(names, got, want):
+            close("d" + k, a, b)
+
+
+def test_broadcast_inputs(dev):
+    """One B, C, dt and state for all samples, one token for all times: expanded views, their gradients summed."""
+    from vit_amd import ssm
+    s = scan_inputs(120, torch.float32, 3, 70, 4, 16, 1, 16, state=True, slices=False)
+    one = dict(s, Bm=s["Bm"][:1], Cm=s["Cm"][:, :1], dt=s["dt"][:1], state=s["state"][:1], z=s["z"][:1, :1])
+    wide = lambda v: {k: t.expand(*s[k].shape) for k, t in v.items()}  # noqa: E731
+    leaf = leaves64(one)
+    wy, _ = ref.selective_scan(**wide(leaf))
+    dy = randn(torch.Generator().manual_seed(4), *wy.shape)
+    want = torch.autograd.grad(wy, list(leaf.values()), dy.double())
+    d = {k: v.to(dev).requires_grad_() for k, v in one.items()}
+    y = _call(ssm, wide(d))
+    close("y", y, wy)
+    for k, a, b in zip(d, torch.autograd.grad(y, list(d.values()), dy.to(dev)), want):
+        close("d" + k, a, b)
+
+
+def test_captured_calls_read_their_lengths_anew(dev):
+    """Two captured graphs (a prompt cut into segments, a convolution with its norms) replayed in turn with other lengths and inputs."""
+    from vit_amd import ssm
+    s = to(scan_inputs(130, torch.bfloat16, 2, 600, 2, 32, 1, 32, state=True), dev)
+    lens = torch.tensor([600, 17], dtype=torch.int32, device=dev)
+    x, w, e = torch.randn(2, 600, 64, device=dev), torch.randn(64, 4, device=dev), torch.ones(64, device=dev)
+
+    def scan():
+        return _call(ssm, s, lengths=lens, return_state=True)
+
+    def conv():
+        u = ssm.causal_conv(x, w, activation="silu", lengths=lens)
+        return ssm.sandwich_norm(x, u, e, None, e, None, gate=e)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        scan(), conv()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for f in (scan, conv):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = f()
+        graphs.append((f, graph, out))
+    for ends in ([600, 17], [0, 600], [513, 512], [1, 64]):
+        lens.copy_(torch.tensor(ends, dtype=torch.int32))
+        x.normal_()
+        for _, graph, _ in graphs:
+            graph.replay()
+        for f, _, out in graphs:
+            for a, b in zip(out, f()):
+                assert torch.equal(a, b), ends
+        torch.cuda.synchronize()
